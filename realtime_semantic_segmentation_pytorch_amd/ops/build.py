@@ -68,6 +68,9 @@ def _kernel_flags():
     return [
         "-c", "-fPIC", "-O3", "-std=c++20", f"--offload-arch={ARCH}", "-mcode-object-version=5",
         "-ffp-contract=fast", "-munsafe-fp-atomics", "-Wno-unused-result",
+        # no v_pk_{add,mul,fma}_f32: some of their operand forms have given wrong results on gfx950
+        # (the host pass does not know the feature and says so; harmless)
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
         "-I", os.path.join(CSRC, "include"),
     ]
 
