@@ -127,6 +127,8 @@ class BaseConfig:
         self.hip_depthwise = True        # depth-wise convs on the HIP kernels (else MIOpen)
         self.hip_pooling = True          # avg / max / adaptive pooling on the HIP kernels
         self.hip_activations = True      # PReLU / ELU / SELU / Hardswish / SiLU / ... on the HIP kernels
+        self.hip_layernorm = True        # layer norms (Mix Transformer encoders) on the HIP kernels, residual sums inside
+        self.act_ckpt8 = False           # hold the activations of linear layers / layer norms for the backward in 8 bits
         self.ddp_bucket_mb = 32          # RCCL all-reduce bucket: ~3 buckets for DDRNet-23 (84 MB), overlapped with backward
         self.ddp_static_graph = True
         self.pg_timeout_s = 600          # collective timeout: a hung rank fails the job (non-zero exit) instead of holding the node

@@ -79,7 +79,7 @@ _SPEC = [
     ("amp_dtype", str, {"choices": ["bf16", "fp16"]}), ("no_channels_last", "true",
                                                         {"dest": "no_channels_last"}),
     ("no_fused_loss", "true", {"dest": "no_fused_loss"}), ("ddp_bucket_mb", int, {}),
-    ("gpu_aug", "true", {}), ("spawn_procs", int, {}), ("graph_step", "true", {}), ("synthetic_data", "true", {}), ("synthetic_len", int, {}),
+    ("gpu_aug", "true", {}), ("spawn_procs", int, {}), ("graph_step", "true", {}), ("act_ckpt8", "true", {}), ("synthetic_data", "true", {}), ("synthetic_len", int, {}),
     ("synthetic_learnable", "true", {}), ("synthetic_cell", int, {}), ("max_train_itrs", int, {}),
     ("cudnn_benchmark", "true", {}), ("deterministic", "true", {}),
     ("log_interval", int, {}), ("device", str, {}),

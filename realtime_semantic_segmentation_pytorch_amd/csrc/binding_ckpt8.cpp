@@ -1,0 +1,351 @@
+// torch.library registration of the layer norm, the 8-bit activation checkpoints and the linear layer
+// that keeps one (layer_norm.hip, ckpt8.hip, linear_ckpt8.hip).
+#include <ATen/ATen.h>
+#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
+#include <torch/library.h>
+
+#include <limits>
+#include <utility>
+
+#include "rtseg_launch.h"
+#include "rtseg_ops.h"
+
+namespace rtseg {
+namespace {
+
+constexpr int64_t kBlock = 32;
+constexpr int64_t kMaxChannels = 1 << 20;  // the kernels' tile counts along channels are grid.y / int
+int64_t padded(int64_t c) { return (c + kBlock - 1) / kBlock * kBlock; }
+
+bool float_type(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf;
+}
+
+// contiguous fp32 / bf16 / fp16 [rows, C] on the GPU
+void check_rows(const at::Tensor& t, const char* op, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && t.is_contiguous() && float_type(t), "rtseg.", op, ": ", what,
+              " must be a contiguous [rows, channels] fp32/bf16/fp16 GPU tensor");
+  TORCH_CHECK(t.size(1) >= 1 && t.size(1) <= kMaxChannels, "rtseg.", op, ": ", what, " needs 1 .. ", kMaxChannels,
+              " channels, got ", t.size(1));
+  TORCH_CHECK(t.size(0) < std::numeric_limits<int>::max(), "rtseg.", op, ": too many rows (", t.size(0), ")");
+}
+
+void check_ckpt(const at::Tensor& codes, const at::Tensor& scales, int64_t rows, int64_t C, const at::Tensor& like,
+                const char* op) {
+  const int64_t Cp = padded(C);
+  TORCH_CHECK(codes.is_cuda() && codes.device() == like.device() && codes.scalar_type() == at::kChar &&
+                  codes.is_contiguous() && codes.dim() == 2 && codes.size(0) == rows && codes.size(1) == Cp,
+              "rtseg.", op, ": codes must be contiguous int8 [", rows, ", ", Cp, "] on the same GPU");
+  TORCH_CHECK(scales.is_cuda() && scales.device() == like.device() && scales.scalar_type() == at::kByte &&
+                  scales.is_contiguous() && scales.dim() == 2 && scales.size(0) == rows && scales.size(1) == Cp / kBlock,
+              "rtseg.", op, ": scales must be contiguous uint8 [", rows, ", ", Cp / kBlock, "] on the same GPU");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0, "rtseg.", op, ": codes must be 16-byte aligned");
+}
+
+std::pair<at::Tensor, at::Tensor> new_ckpt(int64_t rows, int64_t C, const at::Tensor& like) {
+  const int64_t Cp = padded(C);
+  return {at::empty({rows, Cp}, like.options().dtype(at::kChar)),
+          at::empty({rows, Cp / kBlock}, like.options().dtype(at::kByte))};
+}
+
+// a weight or bias vector / matrix: x's type or fp32, contiguous, on x's device
+void check_param(const at::Tensor& t, at::IntArrayRef sizes, const at::Tensor& like, const char* op, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.is_contiguous() && t.sizes() == sizes &&
+                  (t.scalar_type() == like.scalar_type() || t.scalar_type() == at::kFloat),
+              "rtseg.", op, ": ", what, " must be a contiguous ", sizes, " tensor of the input's type or fp32 on its device");
+}
+
+const void* opt_ptr(const std::optional<at::Tensor>& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
+
+// ------------------------------ 8-bit checkpoints -------------------------------
+std::tuple<at::Tensor, at::Tensor> ckpt8_pack(const at::Tensor& x) {
+  check_rows(x, "ckpt8_pack", "x");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  auto [codes, scales] = new_ckpt(x.size(0), x.size(1), x);
+  launch_ckpt8_pack(x.data_ptr(), dtype_code(x), codes.data_ptr<int8_t>(), scales.data_ptr<uint8_t>(), x.size(0),
+                    static_cast<int>(x.size(1)), cur_stream());
+  return {codes, scales};
+}
+
+at::Tensor ckpt8_unpack(const at::Tensor& codes, const at::Tensor& scales, int64_t C, at::ScalarType dtype) {
+  TORCH_CHECK(codes.dim() == 2 && C >= 1 && C <= kMaxChannels,
+              "rtseg.ckpt8_unpack: codes must be [rows, padded channels] with 1 .. ", kMaxChannels, " channels");
+  TORCH_CHECK(codes.size(0) < std::numeric_limits<int>::max(), "rtseg.ckpt8_unpack: too many rows");
+  check_ckpt(codes, scales, codes.size(0), C, codes, "ckpt8_unpack");
+  TORCH_CHECK(dtype == at::kFloat || dtype == at::kBFloat16 || dtype == at::kHalf,
+              "rtseg.ckpt8_unpack: fp32, bf16 or fp16 expected, got ", dtype);
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+  at::Tensor x = at::empty({codes.size(0), C}, codes.options().dtype(dtype));
+  launch_ckpt8_unpack(codes.data_ptr<int8_t>(), scales.data_ptr<uint8_t>(), x.data_ptr(), dtype_code(x), x.size(0),
+                      static_cast<int>(C), cur_stream());
+  return x;
+}
+
+// ------------------------------ layer norm --------------------------------------
+void check_ln_types(int x, int y, const char* op) {
+  TORCH_CHECK(y == x || y == 0 || x == 0, "rtseg.", op, ": the output is of the input's type, fp32, or 16 bits behind fp32");
+}
+
+// keep: 0 nothing, 1 mean / rstd, 2 those and the 8-bit checkpoint.  -> (sum or empty, y, mean, rstd, codes, scales)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
+    const at::Tensor& x, const std::optional<at::Tensor>& r, const std::optional<at::Tensor>& w,
+    const std::optional<at::Tensor>& b, double eps, at::ScalarType out, int64_t keep, bool want_sum) {
+  check_rows(x, "layer_norm", "x");
+  const int64_t rows = x.size(0), C = x.size(1);
+  TORCH_CHECK(C <= layer_norm_max_channels(), "rtseg.layer_norm: at most ", layer_norm_max_channels(), " channels");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  LnFwdArgs a{};
+  a.x = x.data_ptr();
+  a.x_dtype = dtype_code(x);
+  at::Tensor s, y = at::empty({rows, C}, x.options().dtype(out));
+  a.y = y.data_ptr();
+  a.y_dtype = dtype_code(y);
+  check_ln_types(a.x_dtype, a.y_dtype, "layer_norm");
+  if (r.has_value()) {
+    check_rows(*r, "layer_norm", "residual");
+    TORCH_CHECK(r->sizes() == x.sizes() && r->device() == x.device(), "rtseg.layer_norm: residual must match x");
+    a.r = r->data_ptr();
+    a.r_dtype = dtype_code(*r);
+    TORCH_CHECK(a.r_dtype == a.x_dtype || a.x_dtype == 0,
+                "rtseg.layer_norm: residual must be of x's type, or 16 bits beside an fp32 x");
+    if (want_sum) {
+      s = at::empty_like(x);
+      a.s = s.data_ptr();
+    }
+  }
+  for (const auto* p : {&w, &b})
+    if (p->has_value())
+      TORCH_CHECK((*p)->is_cuda() && (*p)->device() == x.device() && (*p)->scalar_type() == at::kFloat &&
+                      (*p)->is_contiguous() && (*p)->dim() == 1 && (*p)->size(0) == C,
+                  "rtseg.layer_norm: weight and bias must be contiguous fp32 [", C, "] on x's device");
+  a.w = static_cast<const float*>(opt_ptr(w));
+  a.b = static_cast<const float*>(opt_ptr(b));
+  at::Tensor mean, rstd, codes, scales;
+  if (keep > 0) {
+    mean = at::empty({rows}, x.options().dtype(at::kFloat));
+    rstd = at::empty_like(mean);
+    a.mean = mean.data_ptr<float>();
+    a.rstd = rstd.data_ptr<float>();
+  }
+  if (keep > 1) {
+    std::tie(codes, scales) = new_ckpt(rows, C, x);
+    a.codes = codes.data_ptr<int8_t>();
+    a.scales = scales.data_ptr<uint8_t>();
+  }
+  a.rows = rows;
+  a.C = static_cast<int>(C);
+  a.Cp = padded(C);
+  a.eps = static_cast<float>(eps);
+  launch_layer_norm_fwd(a, cur_stream());
+  return {s, y, mean, rstd, codes, scales};
+}
+
+// -> (dx or empty, dr, dw, db or empty).  dr is written only where the branch's type is not the
+// stream's: where it is, its gradient is dx.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd(
+    const at::Tensor& dy, const std::optional<at::Tensor>& ds, const std::optional<at::Tensor>& x,
+    const std::optional<at::Tensor>& codes, const std::optional<at::Tensor>& scales, const at::Tensor& mean,
+    const at::Tensor& rstd, const std::optional<at::Tensor>& w, at::ScalarType x_dtype,
+    std::optional<at::ScalarType> r_dtype, bool want_dx, bool want_dr, bool want_w) {
+  check_rows(dy, "layer_norm_bwd", "grad");
+  const int64_t rows = dy.size(0), C = dy.size(1);
+  TORCH_CHECK(C <= layer_norm_max_channels(), "rtseg.layer_norm_bwd: at most ", layer_norm_max_channels(), " channels");
+  TORCH_CHECK(x.has_value() != (codes.has_value() && scales.has_value()),
+              "rtseg.layer_norm_bwd: one of the normalised tensor and its checkpoint");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
+  LnBwdArgs a{};
+  const at::TensorOptions opt = dy.options();
+  at::Tensor dx = at::empty({want_dx ? rows : 0, C}, opt.dtype(x_dtype));
+  a.x_dtype = dtype_code(dx);
+  a.y_dtype = dtype_code(dy);
+  check_ln_types(a.x_dtype, a.y_dtype, "layer_norm_bwd");
+  a.dy = dy.data_ptr();
+  if (x.has_value()) {
+    check_rows(*x, "layer_norm_bwd", "x");
+    TORCH_CHECK(x->sizes() == dy.sizes() && x->device() == dy.device() && x->scalar_type() == x_dtype,
+                "rtseg.layer_norm_bwd: x must match the gradient");
+    a.x = x->data_ptr();
+  } else {
+    check_ckpt(*codes, *scales, rows, C, dy, "layer_norm_bwd");
+    a.codes = codes->data_ptr<int8_t>();
+    a.scales = scales->data_ptr<uint8_t>();
+  }
+  if (ds.has_value()) {
+    check_rows(*ds, "layer_norm_bwd", "gradient of the sum");
+    TORCH_CHECK(ds->sizes() == dy.sizes() && ds->device() == dy.device() && ds->scalar_type() == x_dtype,
+                "rtseg.layer_norm_bwd: the gradient of the sum must be of the sum's shape and type");
+    a.ds = ds->data_ptr();
+  }
+  for (const auto* p : {&mean, &rstd})
+    TORCH_CHECK(p->is_cuda() && p->device() == dy.device() && p->scalar_type() == at::kFloat && p->is_contiguous() &&
+                    p->dim() == 1 && p->size(0) == rows,
+                "rtseg.layer_norm_bwd: mean and rstd must be contiguous fp32 [rows]");
+  a.mean = mean.data_ptr<float>();
+  a.rstd = rstd.data_ptr<float>();
+  if (w.has_value()) {
+    TORCH_CHECK(w->is_cuda() && w->device() == dy.device() && w->scalar_type() == at::kFloat && w->is_contiguous() &&
+                    w->dim() == 1 && w->size(0) == C,
+                "rtseg.layer_norm_bwd: weight must be contiguous fp32 [", C, "]");
+    a.w = w->data_ptr<float>();
+  }
+  a.rows = rows;
+  a.C = static_cast<int>(C);
+  a.Cp = padded(C);
+  at::Tensor dr, dw, db, part;
+  if (want_dr) {
+    TORCH_CHECK(r_dtype.has_value(), "rtseg.layer_norm_bwd: no residual to give a gradient to");
+    TORCH_CHECK(x_dtype == at::kFloat && *r_dtype != x_dtype,
+                "rtseg.layer_norm_bwd: a residual gradient of its own is 16 bits beside an fp32 stream");
+    dr = at::empty({rows, C}, opt.dtype(*r_dtype));
+    a.r_dtype = dtype_code(dr);
+    a.dr = dr.data_ptr();
+  }
+  if (want_dx) a.dx = dx.data_ptr();
+  if (want_w) {
+    dw = at::empty({C}, opt.dtype(at::kFloat));
+    db = at::empty({C}, opt.dtype(at::kFloat));
+    part = at::empty({layer_norm_bwd_blocks(rows, a.C), 2, C}, opt.dtype(at::kFloat));
+    a.part = part.data_ptr<float>();
+  }
+  launch_layer_norm_bwd(a, want_w ? dw.data_ptr<float>() : nullptr, want_w ? db.data_ptr<float>() : nullptr, cur_stream());
+  return {want_dx ? dx : at::Tensor(), dr, dw, db};
+}
+
+// ------------------------------ linear --------------------------------------------
+int act_code(int64_t act) {
+  TORCH_CHECK(act == kCkptNone || act == kCkptGelu, "rtseg.linear_ckpt8: bad activation code ", act);
+  return static_cast<int>(act);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ckpt8_fwd(const at::Tensor& x, const at::Tensor& w,
+                                                                const std::optional<at::Tensor>& b, int64_t act, bool keep) {
+  check_rows(x, "linear_ckpt8", "x");
+  TORCH_CHECK(w.dim() == 2 && w.size(0) >= 1 && w.size(0) <= kMaxChannels,
+              "rtseg.linear_ckpt8: weight must be [out, in] with 1 .. ", kMaxChannels, " outputs");
+  const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+  check_param(w, {N, K}, x, "linear_ckpt8", "weight");
+  if (b.has_value()) {
+    check_param(*b, {N}, x, "linear_ckpt8", "bias");
+    TORCH_CHECK(b->scalar_type() == w.scalar_type(), "rtseg.linear_ckpt8: weight and bias must be of one type");
+  }
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  at::Tensor y = at::empty({M, N}, x.options()), codes, scales;
+  LinFwdArgs a{};
+  if (keep) {
+    std::tie(codes, scales) = new_ckpt(M, K, x);
+    a.codes = codes.data_ptr<int8_t>();
+    a.scales = scales.data_ptr<uint8_t>();
+  }
+  a.x = x.data_ptr();
+  a.w = w.data_ptr();
+  a.b = opt_ptr(b);
+  a.y = y.data_ptr();
+  a.dtype = dtype_code(x);
+  a.w_dtype = dtype_code(w);
+  a.act = act_code(act);
+  a.M = M;
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  launch_lin_fwd(a, cur_stream());
+  return {y, codes, scales};
+}
+
+at::Tensor linear_ckpt8_dgrad(const at::Tensor& dy, const at::Tensor& w, const std::optional<at::Tensor>& codes,
+                              const std::optional<at::Tensor>& scales, int64_t act) {
+  check_rows(dy, "linear_ckpt8_dgrad", "grad");
+  TORCH_CHECK(w.dim() == 2 && w.size(1) >= 1 && w.size(1) <= kMaxChannels,
+              "rtseg.linear_ckpt8_dgrad: weight must be [out, in]");
+  const int64_t M = dy.size(0), N = dy.size(1), K = w.size(1);
+  check_param(w, {N, K}, dy, "linear_ckpt8_dgrad", "weight");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
+  at::Tensor dx = at::empty({M, K}, dy.options());
+  LinDgradArgs a{};
+  a.act = act_code(act);
+  if (a.act != kCkptNone) {
+    TORCH_CHECK(codes.has_value() && scales.has_value(), "rtseg.linear_ckpt8_dgrad: the activation needs the checkpoint");
+    check_ckpt(*codes, *scales, M, K, dy, "linear_ckpt8_dgrad");
+    a.codes = codes->data_ptr<int8_t>();
+    a.scales = scales->data_ptr<uint8_t>();
+  }
+  if (M == 0) return dx;
+  at::Tensor wt = at::empty({K, N}, dy.options());
+  a.dy = dy.data_ptr();
+  a.wt = wt.data_ptr();
+  a.dx = dx.data_ptr();
+  a.dtype = dtype_code(dy);
+  a.M = M;
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  launch_lin_transpose(w.data_ptr(), dtype_code(w), wt.data_ptr(), a.dtype, a.N, a.K, cur_stream());
+  launch_lin_dgrad(a, cur_stream());
+  return dx;
+}
+
+std::tuple<at::Tensor, at::Tensor> linear_ckpt8_wgrad(const at::Tensor& dy, const at::Tensor& codes, const at::Tensor& scales,
+                                                      int64_t K, int64_t act, at::ScalarType w_dtype, bool want_db) {
+  check_rows(dy, "linear_ckpt8_wgrad", "grad");
+  TORCH_CHECK(K >= 1 && K <= kMaxChannels, "rtseg.linear_ckpt8_wgrad: bad input width");
+  const int64_t M = dy.size(0), N = dy.size(1);
+  check_ckpt(codes, scales, M, K, dy, "linear_ckpt8_wgrad");
+  TORCH_CHECK(w_dtype == dy.scalar_type() || w_dtype == at::kFloat,
+              "rtseg.linear_ckpt8_wgrad: the weight is of the gradient's type or fp32");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
+  at::Tensor dw = at::empty({N, K}, dy.options().dtype(w_dtype)), db;
+  if (want_db) db = at::empty({N}, dw.options());
+  LinWgradArgs a{};
+  a.dy = dy.data_ptr();
+  a.codes = codes.data_ptr<int8_t>();
+  a.scales = scales.data_ptr<uint8_t>();
+  a.dw = dw.data_ptr();
+  a.db = want_db ? db.data_ptr() : nullptr;
+  a.dtype = dtype_code(dy);
+  a.w_dtype = dtype_code(dw);
+  a.act = act_code(act);
+  a.M = M;
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  at::Tensor ws = at::empty({lin_wgrad_ws_elems(M, a.N, a.K)}, dy.options().dtype(at::kFloat));
+  a.ws = ws.data_ptr<float>();
+  launch_lin_wgrad(a, cur_stream());
+  return {dw, db};
+}
+
+at::Tensor linear_ckpt8_bgrad(const at::Tensor& dy, at::ScalarType dtype) {
+  check_rows(dy, "linear_ckpt8_bgrad", "grad");
+  TORCH_CHECK(dtype == dy.scalar_type() || dtype == at::kFloat,
+              "rtseg.linear_ckpt8_bgrad: the bias is of the gradient's type or fp32");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
+  at::Tensor db = at::empty({dy.size(1)}, dy.options().dtype(dtype));
+  at::Tensor ws = at::empty({lin_colsum_splits(dy.size(0)) * dy.size(1)}, dy.options().dtype(at::kFloat));
+  launch_lin_colsum(dy.data_ptr(), dtype_code(dy), ws.data_ptr<float>(), db.data_ptr(), dtype_code(db), dy.size(0),
+                    static_cast<int>(dy.size(1)), cur_stream());
+  return db;
+}
+
+}  // namespace
+}  // namespace rtseg
+
+TORCH_LIBRARY_FRAGMENT(rtseg, m) {
+  m.def("ckpt8_pack(Tensor x) -> (Tensor, Tensor)");
+  m.def("ckpt8_unpack(Tensor codes, Tensor scales, int channels, ScalarType dtype) -> Tensor");
+  m.def("layer_norm_fwd(Tensor x, Tensor? r, Tensor? w, Tensor? b, float eps, ScalarType out, int keep, bool want_sum) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("layer_norm_bwd(Tensor dy, Tensor? ds, Tensor? x, Tensor? codes, Tensor? scales, Tensor mean, Tensor rstd, Tensor? w, "
+        "ScalarType x_dtype, ScalarType? r_dtype, bool want_dx, bool want_dr, bool want_w) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("linear_ckpt8_fwd(Tensor x, Tensor w, Tensor? b, int act, bool keep) -> (Tensor, Tensor, Tensor)");
+  m.def("linear_ckpt8_dgrad(Tensor dy, Tensor w, Tensor? codes, Tensor? scales, int act) -> Tensor");
+  m.def("linear_ckpt8_wgrad(Tensor dy, Tensor codes, Tensor scales, int K, int act, ScalarType w_dtype, bool want_db) -> "
+        "(Tensor, Tensor)");
+  m.def("linear_ckpt8_bgrad(Tensor dy, ScalarType dtype) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(rtseg, CUDA, m) {
+  m.impl("ckpt8_pack", &rtseg::ckpt8_pack);
+  m.impl("ckpt8_unpack", &rtseg::ckpt8_unpack);
+  m.impl("layer_norm_fwd", &rtseg::layer_norm_fwd);
+  m.impl("layer_norm_bwd", &rtseg::layer_norm_bwd);
+  m.impl("linear_ckpt8_fwd", &rtseg::linear_ckpt8_fwd);
+  m.impl("linear_ckpt8_dgrad", &rtseg::linear_ckpt8_dgrad);
+  m.impl("linear_ckpt8_wgrad", &rtseg::linear_ckpt8_wgrad);
+  m.impl("linear_ckpt8_bgrad", &rtseg::linear_ckpt8_bgrad);
+}

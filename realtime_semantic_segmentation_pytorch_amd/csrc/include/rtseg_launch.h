@@ -434,4 +434,104 @@ void launch_act(const ActArgs& a, hipStream_t st);
 enum ShufMode : int { kShufPixel = 0, kShufPixelInv = 1, kShufChannel = 2 };
 void launch_shuffle(const Tensor4& in, const Tensor4& out, int mode, int r, bool out_cl, hipStream_t st);
 
+// ---- ckpt8.hip ------------------------------------------------------------------
+// 8-bit activation checkpoints (format: rtseg_ckpt8.h): x [rows, C] contiguous fp32 / bf16 / fp16,
+// codes int8 [rows, Cp], scales uint8 [rows, Cp / 32], Cp = C rounded up to 32; codes 8-byte aligned.
+void launch_ckpt8_pack(const void* x, int dtype, int8_t* codes, uint8_t* scales, int64_t rows, int C, hipStream_t st);
+void launch_ckpt8_unpack(const int8_t* codes, const uint8_t* scales, void* x, int dtype, int64_t rows, int C,
+                         hipStream_t st);
+
+// ---- layer_norm.hip ---------------------------------------------------------------
+// All tensors are contiguous [rows, C]; 1 <= C <= layer_norm_max_channels().  The output type is the
+// stream's, fp32, or 16 bits behind an fp32 stream; the branch r is of the stream's type, or 16 bits
+// behind an fp32 stream.
+struct LnFwdArgs {
+  const void* x;
+  const void* r;      // branch added in front, or nullptr
+  void* s;            // x + r, or nullptr (no branch, or the sum is not wanted)
+  void* y;
+  const float* w;     // [C] or nullptr
+  const float* b;     // [C] or nullptr
+  float* mean;        // [rows] or nullptr (inference)
+  float* rstd;
+  int8_t* codes;      // 8-bit checkpoint of the normalised tensor, or nullptr
+  uint8_t* scales;
+  int x_dtype, r_dtype, y_dtype;
+  int64_t rows;
+  int C;
+  int64_t Cp;
+  float eps;
+  int lanes;          // set by the launcher
+  bool vec, wvec;
+};
+struct LnBwdArgs {
+  const void* dy;
+  const void* ds;     // gradient of the sum (the stream's type), or nullptr
+  const void* x;      // the normalised tensor, or nullptr with codes
+  const int8_t* codes;
+  const uint8_t* scales;
+  const float* mean;
+  const float* rstd;
+  const float* w;     // [C] or nullptr
+  void* dx;           // the stream's type, or nullptr
+  void* dr;           // r_dtype, or nullptr (none, or the same tensor as dx)
+  float* part;        // [layer_norm_bwd_blocks, 2, C] or nullptr (no weight gradients wanted)
+  int x_dtype, r_dtype, y_dtype;
+  int64_t rows;
+  int C;
+  int64_t Cp;
+  int lanes, blocks;  // set by the launcher
+  bool vec, wvec;
+};
+int layer_norm_max_channels();
+int layer_norm_bwd_blocks(int64_t rows, int C);
+void launch_layer_norm_fwd(LnFwdArgs a, hipStream_t st);
+void launch_layer_norm_bwd(LnBwdArgs a, float* dw, float* db, hipStream_t st);
+
+// ---- linear_ckpt8.hip ---------------------------------------------------------------
+// y = act(x) w^T + b for x [M, K], w [N, K]; the checkpoint of x is written by the forward and read by
+// both gradients.  x / y / dy / dx are of one type (fp32 / bf16 / fp16); w and b that type or fp32.
+enum CkptAct : int { kCkptNone = 0, kCkptGelu = 1 };
+struct LinFwdArgs {
+  const void* x;
+  const void* w;
+  const void* b;      // [N] of w's type, or nullptr
+  void* y;
+  int8_t* codes;      // or nullptr: nothing is kept
+  uint8_t* scales;
+  int dtype, w_dtype, act;
+  int64_t M;
+  int N, K;
+};
+struct LinDgradArgs {
+  const void* dy;     // [M, N]
+  const void* wt;     // [K, N], w transposed, of dy's type
+  const int8_t* codes;  // read with act != none only
+  const uint8_t* scales;
+  void* dx;           // [M, K]
+  int dtype, act;
+  int64_t M;
+  int N, K;
+};
+struct LinWgradArgs {
+  const void* dy;
+  const int8_t* codes;
+  const uint8_t* scales;
+  float* ws;          // lin_wgrad_ws_elems
+  void* dw;           // [N, K], or nullptr
+  void* db;           // [N], or nullptr
+  int dtype, w_dtype, act;
+  int64_t M;
+  int N, K;
+};
+void launch_lin_fwd(const LinFwdArgs& a, hipStream_t st);
+// wt [K, N] (dtype) = w [N, K] (w_dtype) transposed
+void launch_lin_transpose(const void* w, int w_dtype, void* wt, int dtype, int N, int K, hipStream_t st);
+void launch_lin_dgrad(const LinDgradArgs& a, hipStream_t st);
+int64_t lin_wgrad_ws_elems(int64_t M, int N, int K);
+void launch_lin_wgrad(const LinWgradArgs& a, hipStream_t st);
+// db [N] = column sums of dy [M, N]; ws: lin_colsum_splits(M) * N floats
+int lin_colsum_splits(int64_t M);
+void launch_lin_colsum(const void* dy, int dtype, float* ws, void* db, int db_dtype, int64_t M, int N, hipStream_t st);
+
 }  // namespace rtseg

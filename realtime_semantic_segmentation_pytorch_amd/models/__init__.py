@@ -89,6 +89,10 @@ def get_model(config):
     if getattr(config, "hip_activations", True):
         ops.convert_activations(model)
     ops.convert_pixel_shuffle(model)
+    if getattr(config, "hip_layernorm", True):
+        ops.convert_layernorm(model)
+    if getattr(config, "act_ckpt8", False):
+        ops.convert_ckpt8(model)  # linear layers, layer norms, Mix Transformer convs: saved activations in 8 bits
     return model
 
 

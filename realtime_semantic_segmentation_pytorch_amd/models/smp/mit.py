@@ -13,7 +13,11 @@ returns ``[x, empty(B, 0, H/2, W/2), f4, f8, f16, f32]`` -- the zero-channel str
 is SMP's placeholder for the stage MiT does not have.
 
 MI355X notes: attention runs through ``F.scaled_dot_product_attention`` (the fused ROCm flash
-kernels); the spatial-reduction conv and the Mix-FFN depth-wise conv are channels-last convs.
+kernels); the spatial-reduction conv and the Mix-FFN depth-wise conv are channels-last convs.  With
+``ops.convert_layernorm`` (``config.hip_layernorm``) every residual sum runs inside the norm behind it,
+which writes the next linear layer's type at once; with ``ops.convert_ckpt8`` (``config.act_ckpt8``) the
+activations held for the backward are 8-bit checkpoints, the Mix-FFN's GELU inside its second linear
+layer.
 """
 from __future__ import annotations
 
@@ -22,6 +26,8 @@ import math
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ... import ops
 
 # name: (embed_dims, depths); every variant: heads (1, 2, 5, 8), sr (8, 4, 2, 1), mlp ratio 4
 MIT_SPECS = {
@@ -44,6 +50,19 @@ def _drop_path(x, p, training):
     return x * mask / keep
 
 
+def _add_norm(norm, x, branch=None, cast=True, want_sum=True):
+    """``(s, norm(s))`` for ``s = x + branch``; on the HIP kernel one pass, whose result has the type that
+    the linear layers behind it run in (``cast``; autocast would convert it there)."""
+    if isinstance(norm, ops.LayerNorm) and (x.is_cuda or norm.ckpt8):
+        kind = x.device.type
+        out = torch.get_autocast_dtype(kind) if cast and torch.is_autocast_enabled(kind) else None
+        if branch is None:
+            return x, norm(x, out_dtype=out)
+        return norm(x, residual=branch, out_dtype=out, want_sum=want_sum)
+    x = x if branch is None else x + branch
+    return x, norm(x)
+
+
 class DropPath(nn.Module):
     def __init__(self, p=0.0):
         super().__init__()
@@ -54,6 +73,8 @@ class DropPath(nn.Module):
 
 
 class DWConv(nn.Module):
+    ckpt8 = False  # hold the conv's input in 8 bits (ops.convert_ckpt8)
+
     def __init__(self, dim):
         super().__init__()
         self.dwconv = nn.Conv2d(dim, dim, 3, 1, 1, bias=True, groups=dim)
@@ -61,7 +82,9 @@ class DWConv(nn.Module):
     def forward(self, x, h, w):
         b, n, c = x.shape
         x = x.transpose(1, 2).reshape(b, c, h, w)
-        return self.dwconv(x).flatten(2).transpose(1, 2)
+        with ops.ckpt8_saved(x if self.ckpt8 else None):
+            y = self.dwconv(x)
+        return y.flatten(2).transpose(1, 2)
 
 
 class Mlp(nn.Module):
@@ -73,11 +96,16 @@ class Mlp(nn.Module):
         self.fc2 = nn.Linear(hidden, dim)
 
     def forward(self, x, h, w):
-        return self.fc2(self.act(self.dwconv(self.fc1(x), h, w)))
+        x = self.dwconv(self.fc1(x), h, w)
+        if isinstance(self.fc2, ops.Ckpt8Linear) and isinstance(self.act, nn.GELU) and self.act.approximate == "none":
+            return self.fc2(x, act="gelu")
+        return self.fc2(self.act(x))
 
 
 class Attention(nn.Module):
     """Efficient self-attention: keys / values from a sr x sr strided-conv reduced sequence."""
+
+    ckpt8 = False  # hold the spatial-reduction conv's input in 8 bits (ops.convert_ckpt8)
 
     def __init__(self, dim, num_heads, sr_ratio):
         super().__init__()
@@ -97,8 +125,10 @@ class Attention(nn.Module):
         nh = self.num_heads
         q = self.q(x).reshape(b, n, nh, c // nh).transpose(1, 2)
         if self.sr_ratio > 1:
-            xs = self.sr(x.transpose(1, 2).reshape(b, c, h, w)).flatten(2).transpose(1, 2)
-            xs = self.norm(xs)
+            xs = x.transpose(1, 2).reshape(b, c, h, w)
+            with ops.ckpt8_saved(xs if self.ckpt8 else None):
+                xs = self.sr(xs)
+            xs = _add_norm(self.norm, xs.flatten(2).transpose(1, 2))[1]
         else:
             xs = x
         kv = self.kv(xs).reshape(b, -1, 2, nh, c // nh).permute(2, 0, 3, 1, 4)
@@ -115,9 +145,13 @@ class Block(nn.Module):
         self.norm2 = nn.LayerNorm(dim, eps=1e-6)
         self.mlp = Mlp(dim, dim * 4)
 
-    def forward(self, x, h, w):
-        x = x + self.drop_path(self.attn(self.norm1(x), h, w))
-        return x + self.drop_path(self.mlp(self.norm2(x), h, w))
+    def forward(self, x, h, w, branch=None, split=False):
+        """``branch`` is added to ``x`` first; ``split`` returns (stream, its last branch) unadded, so
+        that the next norm adds them."""
+        x, y = _add_norm(self.norm1, x, branch)
+        x, y = _add_norm(self.norm2, x, self.drop_path(self.attn(y, h, w)))
+        branch = self.drop_path(self.mlp(y, h, w))
+        return (x, branch) if split else x + branch
 
 
 class OverlapPatchEmbed(nn.Module):
@@ -165,9 +199,10 @@ class MixVisionTransformerEncoder(nn.Module):
         outs = []
         for i in range(1, 5):
             x, h, w = getattr(self, f"patch_embed{i}")(x)
+            branch = None
             for blk in getattr(self, f"block{i}"):
-                x = blk(x, h, w)
-            x = getattr(self, f"norm{i}")(x)
+                x, branch = blk(x, h, w, branch, True)
+            _, x = _add_norm(getattr(self, f"norm{i}"), x, branch, cast=False, want_sum=False)
             x = x.reshape(b, h, w, -1).permute(0, 3, 1, 2).contiguous()
             outs.append(x)
         return outs

@@ -31,6 +31,9 @@ from .act import activation, convert_activations
 from .shuffle import channel_shuffle, convert_pixel_shuffle, pixel_shuffle, pixel_unshuffle
 from .augment import AugmentSpec, augment_batch, augment_reference, draw_params
 from .streams import concurrent_branches
+from .layer_norm import layer_norm, layer_norm_reference, LayerNorm, convert_layernorm
+from .ckpt8 import (Ckpt8, ckpt8_pack, ckpt8_unpack, ckpt8_saved, linear_ckpt8, linear_ckpt8_reference, Ckpt8Linear,
+                    convert_ckpt8)
 
 __all__ = [
     "load", "use_hip", "hip_disabled", "library_path",
@@ -45,4 +48,5 @@ __all__ = [
     "FusedSGD", "FusedAdam", "FusedAdamW", "conv_ok", "conv_bn_stats", "stem_store_skippable", "twin_conv_bn_stats", "conv_bn_act_eval", "conv_bn_act", "conv_forward", "RoutedConv2d", "GroupedConv2d", "convert_routed_convs", "invalidate_weight_shadows",
     "TransposedConv2d", "conv_transpose2d", "convert_transposed_convs", "deconv_ok", "gate", "gate_reference", "activation", "convert_activations", "channel_shuffle", "convert_pixel_shuffle", "pixel_shuffle", "pixel_unshuffle", "AugmentSpec", "augment_batch", "augment_reference", "draw_params",
     "concurrent_branches", "ConcatSink", "cat_bn_act", "bn_act", "bn_stats_begin", "bias_add", "bn_act_code", "bn_fused_ok", "convert_batchnorm", "FusedBatchNorm2d", "FusedSyncBatchNorm",
+    "layer_norm", "layer_norm_reference", "LayerNorm", "convert_layernorm", "Ckpt8", "ckpt8_pack", "ckpt8_unpack", "ckpt8_saved", "linear_ckpt8", "linear_ckpt8_reference", "Ckpt8Linear", "convert_ckpt8",
 ]

@@ -73,8 +73,8 @@ def library_path() -> str:
 
 def families_off() -> frozenset:
     """``RTSEG_HIP_OFF=bn,interp,...``: kernel families sent to their stock PyTorch formulation
-    (numerics bisection, tools/probe_numerics_bisect.py).  Families: act, bn, conv, deconv, detail,
-    dilated, dw, gate, interp, kd, loss, pool, shuffle, tapconv."""
+    (numerics bisection, tools/probe_numerics_bisect.py).  Families: act, bn, ckpt8, conv, deconv,
+    detail, dilated, dw, gate, interp, kd, layer_norm, loss, pool, shuffle, tapconv."""
     raw = os.environ.get("RTSEG_HIP_OFF", "")
     return frozenset(f.strip() for f in raw.split(",") if f.strip())
 

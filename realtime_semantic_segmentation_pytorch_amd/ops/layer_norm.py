@@ -1,0 +1,209 @@
+"""Layer norm over the last axis on the HIP kernels of ``csrc/kernels/layer_norm.hip``.
+
+Reference: the Mix Transformer encoders that the reference reaches through
+segmentation_models_pytorch (reference models/__init__.py:67-81) normalise every token of the
+residual stream twice per block (``nn.LayerNorm``).  Here the sum of the residual stream and a
+branch, the norm and the cast to the next linear layer's type are one pass, and the backward is one
+pass that also adds the stream's own gradient and reduces the weight gradients (fp32, without
+atomics: the same bits on every run).
+
+``ckpt8=True`` holds the normalised tensor for the backward as an 8-bit checkpoint (``ops.ckpt8``)
+instead of the tensor itself.  CPU tensors, ``RTSEG_DISABLE_HIP=1`` / ``RTSEG_HIP_OFF=layer_norm``
+and more than 8192 channels run the same formulas in PyTorch.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from ._ext import ops, use_hip
+
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_MAX_CHANNELS = 8192  # a row is held in one block's registers
+
+
+def _autocast_dtype(t: torch.Tensor) -> Optional[torch.dtype]:
+    kind = t.device.type
+    return torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else None
+
+
+def _default_out(x: torch.Tensor) -> torch.dtype:
+    """What ``F.layer_norm`` returns: fp32 under autocast, else the input's type."""
+    return torch.float32 if _autocast_dtype(x) is not None else x.dtype
+
+
+def layer_norm_reference(x, weight=None, bias=None, eps=1e-5, residual=None, out_dtype=None):
+    """The formulas of :func:`layer_norm` in PyTorch (statistics in fp32, or in fp64 for fp64 inputs)."""
+    out_dtype = out_dtype or x.dtype
+    s = x if residual is None else x + residual
+    wide = s.dtype if s.dtype == torch.float64 else torch.float32
+    with torch.autocast(s.device.type, enabled=False):
+        y = F.layer_norm(s.to(wide), s.shape[-1:], None if weight is None else weight.to(wide),
+                         None if bias is None else bias.to(wide), eps).to(out_dtype)
+    return y if residual is None else (s, y)
+
+
+class _LayerNormFn(torch.autograd.Function):
+    """(x, residual | None) -> y, or (x + residual, y)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, out_dtype, ckpt8, want_sum):
+        shape, c = x.shape, x.shape[-1]
+        x2 = x.reshape(-1, c).contiguous()
+        r2 = None if residual is None else residual.reshape(-1, c).contiguous()
+        w = None if weight is None else weight.detach().float().contiguous()
+        b = None if bias is None else bias.detach().float().contiguous()
+        train = any(ctx.needs_input_grad)
+        keep = (2 if ckpt8 else 1) if train else 0
+        # without a checkpoint the backward normalises the sum again, so it is kept even if unwanted
+        s, y, mean, rstd, codes, scales = ops().layer_norm_fwd(x2, r2, w, b, eps, out_dtype, keep,
+                                                               want_sum or keep == 1)
+        ctx.set_materialize_grads(False)
+        if train:
+            ctx.shape, ctx.types = shape, (x.dtype, None if residual is None else residual.dtype)
+            ctx.param_types = (weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
+            kept = (codes, scales) if ckpt8 else (x2 if residual is None else s, None)
+            ctx.save_for_backward(*kept, mean, rstd, w)
+        y = y.view(shape)
+        return (s.view(shape) if want_sum else None), y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, ds, dy):
+        first, scales, mean, rstd, w = ctx.saved_tensors
+        shape, (xt, rt) = ctx.shape, ctx.types
+        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
+        if dy is None:  # the norm's output is unused: only the sum carries a gradient
+            gx = ds if need_x else None
+            gr = ds.to(rt) if (need_r and ds is not None) else None
+            return gx, gr, None, None, None, None, None, None
+        c = shape[-1]
+        dy = dy.reshape(-1, c).contiguous()
+        ds = None if ds is None else ds.reshape(-1, c).contiguous()
+        x, codes = (first, None) if scales is None else (None, first)
+        own_r = need_r and rt != xt
+        dx, dr, dw, db = ops().layer_norm_bwd(dy, ds, x, codes, scales, mean, rstd, w, xt, rt,
+                                              need_x or (need_r and not own_r), own_r, need_w or need_b)
+        dx = None if dx is None else dx.view(shape)
+        gr = None if not need_r else (dr.view(shape) if own_r else dx)
+        wt, bt = ctx.param_types
+        return (dx if need_x else None, gr, dw.to(wt) if need_w else None, db.to(bt) if need_b else None,
+                None, None, None, None)
+
+
+class _LayerNormCkptFn(torch.autograd.Function):
+    """The PyTorch formulation with an 8-bit checkpoint (CPU tensors)."""
+
+    @staticmethod
+    def forward(ctx, s, weight, bias, eps, out_dtype):
+        from .ckpt8 import ckpt8_pack
+
+        wide = s.detach().float()
+        mean = wide.mean(-1, keepdim=True)
+        rstd = torch.rsqrt((wide - mean).square().mean(-1, keepdim=True) + eps)
+        h = (wide - mean) * rstd
+        if weight is not None:
+            h = h * weight.float()
+        if bias is not None:
+            h = h + bias.float()
+        kept = ckpt8_pack(s.detach())
+        ctx.kept = kept._replace(codes=None, scales=None)
+        ctx.save_for_backward(kept.codes, kept.scales, mean, rstd, weight)
+        ctx.bias_type = None if bias is None else bias.dtype
+        return h.to(out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        from .ckpt8 import ckpt8_unpack
+
+        codes, scales, mean, rstd, weight = ctx.saved_tensors
+        x = ckpt8_unpack(ctx.kept._replace(codes=codes, scales=scales))
+        h = (x.float() - mean) * rstd
+        dy = dy.float()
+        g = dy if weight is None else dy * weight.float()
+        dx = rstd * (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True))
+        lead = tuple(range(dy.dim() - 1))
+        return (dx.to(x.dtype) if ctx.needs_input_grad[0] else None,
+                (dy * h).sum(lead).to(weight.dtype) if ctx.needs_input_grad[1] else None,
+                dy.sum(lead).to(ctx.bias_type) if ctx.needs_input_grad[2] else None, None, None)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, residual: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+               ckpt8: bool = False, want_sum: bool = True):
+    """``y = (s - mean) * rsqrt(var + eps) * weight + bias`` over the last axis, ``s = x``; with
+    ``residual`` the pair ``(s, y)`` for ``s = x + residual`` (``want_sum=False``: ``(None, y)``).
+
+    ``x``: ``[..., C]`` fp32 / bf16 / fp16, any strides (a non-contiguous one is copied once).  ``s``
+    has the promoted type of ``x`` and ``residual``; ``y`` has ``out_dtype``, by default fp32 under
+    autocast and the type of ``s`` otherwise (as ``F.layer_norm``).  ``weight`` / ``bias``: ``[C]`` or
+    None, applied in fp32.  ``ckpt8``: hold ``s`` for the backward in 8 bits; the backward then uses
+    the checkpoint's values in place of ``s`` (with the exact mean and variance).
+    """
+    c = x.shape[-1] if x.dim() else 0
+    if c < 1:
+        raise ValueError(f"layer_norm: the last axis must have at least one channel, got shape {tuple(x.shape)}")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and tuple(p.shape) != (c,):
+            raise ValueError(f"layer_norm: {name} must have shape ({c},), got {tuple(p.shape)}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"layer_norm: residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if out_dtype is not None and not out_dtype.is_floating_point:
+        raise ValueError(f"layer_norm: out_dtype must be a floating type, got {out_dtype}")
+    if residual is not None:
+        wide = torch.promote_types(x.dtype, residual.dtype)
+        if x.dtype != wide:
+            x = x.to(wide)
+        # an fp32 stream takes a 16-bit branch as it is; every other pair is added in one type
+        if residual.dtype != wide and not (wide == torch.float32 and residual.dtype in _DTYPES):
+            residual = residual.to(wide)
+    out_dtype = out_dtype or _default_out(x)
+    if x.dtype in _DTYPES and out_dtype in _DTYPES and c <= _MAX_CHANNELS and use_hip(x, "layer_norm"):
+        # 16 bits in and another 16-bit type out: through fp32
+        got = out_dtype if out_dtype == x.dtype or torch.float32 in (out_dtype, x.dtype) else torch.float32
+        s, y = _LayerNormFn.apply(x, residual, weight, bias, float(eps), got, bool(ckpt8), residual is not None and want_sum)
+        y = y if got == out_dtype else y.to(out_dtype)
+        return y if residual is None else (s, y)
+    if ckpt8 and x.dtype in _DTYPES and torch.is_grad_enabled():
+        s = x if residual is None else x + residual
+        y = _LayerNormCkptFn.apply(s, weight, bias, float(eps), out_dtype)
+        return y if residual is None else (s if want_sum else None, y)
+    got = layer_norm_reference(x, weight, bias, eps, residual, out_dtype)
+    return got if residual is None or want_sum else (None, got[1])
+
+
+class LayerNorm(nn.LayerNorm):
+    """``nn.LayerNorm`` over one axis on :func:`layer_norm`; parameters and state_dict keys unchanged.
+
+    ``forward(x)`` is the stock module's.  ``forward(x, residual=r)`` returns ``(x + r, norm(x + r))``,
+    ``out_dtype`` sets the result's type, and ``ckpt8`` (an attribute, off) holds the normalised tensor
+    in 8 bits for the backward."""
+
+    ckpt8 = False
+
+    def forward(self, x, residual=None, out_dtype=None, want_sum=True):
+        if len(self.normalized_shape) != 1:
+            if residual is not None or out_dtype is not None:
+                raise ValueError("LayerNorm: residual / out_dtype need a norm over the last axis alone")
+            return super().forward(x)
+        if x.shape[-1] != self.normalized_shape[0]:
+            raise ValueError(f"LayerNorm: {self.normalized_shape[0]} channels expected, got shape {tuple(x.shape)}")
+        if x.device.type != "cuda" and residual is None and out_dtype is None and not self.ckpt8:
+            return super().forward(x)
+        return layer_norm(x, self.weight, self.bias, self.eps, residual, out_dtype, self.ckpt8, want_sum)
+
+
+def convert_layernorm(model: nn.Module) -> nn.Module:
+    """Swap every ``nn.LayerNorm`` of ``model`` onto :class:`LayerNorm` (in place)."""
+    for m in model.modules():
+        if type(m) is nn.LayerNorm:
+            m.__class__ = LayerNorm
+    return model
+
+
+__all__ = ["layer_norm", "layer_norm_reference", "LayerNorm", "convert_layernorm"]
