@@ -268,15 +268,14 @@ at::Tensor linear_ckpt8_dgrad(const at::Tensor& dy, const at::Tensor& w, const s
     a.scales = scales->data_ptr<uint8_t>();
   }
   if (M == 0) return dx;
-  at::Tensor wt = at::empty({K, N}, dy.options());
   a.dy = dy.data_ptr();
-  a.wt = wt.data_ptr();
+  a.w = w.data_ptr();
+  a.w_dtype = dtype_code(w);
   a.dx = dx.data_ptr();
   a.dtype = dtype_code(dy);
   a.M = M;
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
-  launch_lin_transpose(w.data_ptr(), dtype_code(w), wt.data_ptr(), a.dtype, a.N, a.K, cur_stream());
   launch_lin_dgrad(a, cur_stream());
   return dx;
 }

@@ -505,11 +505,11 @@ struct LinFwdArgs {
 };
 struct LinDgradArgs {
   const void* dy;     // [M, N]
-  const void* wt;     // [K, N], w transposed, of dy's type
+  const void* w;      // [N, K]
   const int8_t* codes;  // read with act != none only
   const uint8_t* scales;
   void* dx;           // [M, K]
-  int dtype, act;
+  int dtype, w_dtype, act;
   int64_t M;
   int N, K;
 };
@@ -525,8 +525,6 @@ struct LinWgradArgs {
   int N, K;
 };
 void launch_lin_fwd(const LinFwdArgs& a, hipStream_t st);
-// wt [K, N] (dtype) = w [N, K] (w_dtype) transposed
-void launch_lin_transpose(const void* w, int w_dtype, void* wt, int dtype, int N, int K, hipStream_t st);
 void launch_lin_dgrad(const LinDgradArgs& a, hipStream_t st);
 int64_t lin_wgrad_ws_elems(int64_t M, int N, int K);
 void launch_lin_wgrad(const LinWgradArgs& a, hipStream_t st);

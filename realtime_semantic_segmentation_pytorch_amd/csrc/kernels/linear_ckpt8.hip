@@ -30,9 +30,34 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float gelu(float x) { return 0.5f * x * (1.f + erff(x * 0.70710678118654752f)); }
+// Phi(-|x|), the normal tail, by Abramowitz and Stegun 7.1.26 (erfc(z) = t (a1 + ... + a5 t^4) exp(-z^2),
+// t = 1 / (1 + p z), error below 1.5e-7) with z = |x| / sqrt(2) folded into the constants; e = exp(-x^2 / 2)
+__device__ __forceinline__ float normal_tail(float ax, float e) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(ax, 0.3275911f * 0.70710678118654752f, 1.f));
+  float q = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  q = __builtin_fmaf(t, q, 0.5f * 1.421413741f);
+  q = __builtin_fmaf(t, q, 0.5f * -0.284496736f);
+  q = __builtin_fmaf(t, q, 0.5f * 0.254829592f);
+  return q * t * e;
+}
+__device__ __forceinline__ float exp_half_square(float x) {  // exp(-x^2 / 2)
+  return __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f);
+}
+// gelu(x) = x Phi(x) = max(x, 0) - |x| Phi(-|x|), gelu'(x) = Phi(x) + x phi(x).  16-bit operands take the tail
+// above (14 full-rate and 2 quarter-rate instructions, 0.75e-7 |x| off, far below their rounding: a fifth of
+// erff's cost, which bound all three products); fp32 ones erff.
+template <typename T>
+__device__ __forceinline__ float gelu(float x) {
+  if constexpr (sizeof(T) == 4) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+  const float ax = fabsf(x);  // the factor is cut off where the tail is 0: inf - inf * 0 is inf
+  return __builtin_fmaf(-fminf(ax, 64.f), normal_tail(ax, exp_half_square(x)), fmaxf(x, 0.f));
+}
+template <typename T>
 __device__ __forceinline__ float gelu_slope(float x) {
-  return 0.5f * (1.f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * __expf(-0.5f * x * x);
+  if constexpr (sizeof(T) == 4)
+    return 0.5f * (1.f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * __expf(-0.5f * x * x);
+  const float e = exp_half_square(x), tail = normal_tail(fabsf(x), e);
+  return __builtin_fmaf(x * 0.39894228040143268f, e, x >= 0.f ? 1.f - tail : tail);
 }
 
 // 16 bytes of operand: 8 (bf16 / fp16) or 4 (fp32) consecutive k
@@ -60,21 +85,31 @@ __device__ __forceinline__ uint4 pack16<uint16_t>(const float* v) {
                     f32x2_to_bf16x2(v[6], v[7]));
 }
 
-// 16 bytes of T from p; n: elements from p on that exist; vec: p is 16-byte aligned and n <= 0 or whole
-template <typename T>
-__device__ __forceinline__ uint4 load16(const T* p, int n, bool vec) {
-  uint4 q = make_uint4(0u, 0u, 0u, 0u);
-  if (vec) {
-    if (n > 0) q = *reinterpret_cast<const uint4*>(p);
-  } else {
-    T t[kPer16<T>];
+// A range of a tensor as a buffer: accesses past `bytes` read 0, so a tile's missing rows cost no branch.
+// kOut as an offset is past every range.
+constexpr uint32_t kOut = 0xfffffff0u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t range(const void* p, int64_t bytes) {
+  const uint32_t n = bytes < 0 ? 0u : bytes > 0xffffff00ll ? 0xffffff00u : static_cast<uint32_t>(bytes);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(n), 0x00020000);
+}
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 buf16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(uint4, static_cast<u32x4_t>(__builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(off), 0, 0)));
+}
+// 16 bytes of T at byte offset off, of which the first n elements exist (n <= 0: none); VEC: off is
+// 16-byte aligned and n is <= 0 or whole
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off, int n) {
+  if constexpr (VEC) return buf16(r, n > 0 ? off : kOut);
+  T t[kPer16<T>];
 #pragma unroll
-    for (int i = 0; i < kPer16<T>; ++i) {
-      t[i] = T(0);
-      if (i < n) t[i] = p[i];
-    }
-    __builtin_memcpy(&q, t, 16);
+  for (int i = 0; i < kPer16<T>; ++i) {
+    const int o = static_cast<int>(i < n ? off + i * sizeof(T) : kOut);
+    if constexpr (sizeof(T) == 4) t[i] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0));
+    else t[i] = __builtin_bit_cast(T, static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0)));
   }
+  uint4 q;
+  __builtin_memcpy(&q, t, 16);
   return q;
 }
 
@@ -98,64 +133,89 @@ __device__ __forceinline__ f32x4_t mma16(uint4 a, uint4 b, f32x4_t c) {
 
 // ------------------------------------------------------------------------------- forward, dgrad
 struct NtArgs {
-  const void* a;        // [M, K]
-  const void* b;        // [N, K]
-  const void* bias;     // [N] of b's type, or nullptr
+  const void* a;        // [M, K]: x, or dy
+  const void* w;        // forward [N, K]; dgrad [K, N]
+  const void* bias;     // [N] of w's type, or nullptr
   void* out;            // [M, N]
   int8_t* codes;        // forward: written, of a; dgrad with gelu: read, of out
   uint8_t* scales;
   int64_t M;
   int N, K, Cp;         // Cp: columns of codes
   int ntiles;           // column tiles
-  bool b_f32;           // b (and bias) are fp32 beside 16-bit operands
-  bool va, vb, vo;      // 16-byte accesses to a / b / out
+  bool w_f32;           // w (and bias) are fp32 beside 16-bit operands
+  bool vo;              // 16-byte stores to out
 };
 
-// LDS rows are 8 chunks of 16 bytes.  Row operand (weights): lane r of a fragment reads row
-// 16 * (r / 4) + 4 * t + r % 4; column operand: row 16 * t + r.  The chunk index is XORed so that the
-// rows of one read spread over the banks.
+__device__ __forceinline__ uint2 tr_read(const void* p) {
+  auto q = (__attribute__((address_space(3))) mdev::i16x4_t*)((__attribute__((address_space(3))) void*)const_cast<void*>(p));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(q));
+}
+
+// A lane of a fragment ends with columns 16 g .. 16 g + 15 of its wave's 64 (g = lane / 16): row r of the
+// row operand's tile t is column 16 (r / 4) + 4 t + r % 4, for fp32 in dgrad 4 r + t.
+//
+// LDS.  a: rows of 8 chunks of 16 bytes, chunk ^ (row & 7).  Forward w, the same, with the XOR taken from
+// the row bits that one fragment read runs over.  dgrad w: BK rows of BN columns as in memory, read
+// transposed: 8-byte units, XORed with row & 3 (a 16-lane group reads 4 rows) and row bit 3 (two groups).
+__device__ __forceinline__ int swz_a(int row) { return row & 7; }
 __device__ __forceinline__ int swz_w(int row) { return (row & 3) | ((row >> 4) & 1) << 2; }
-__device__ __forceinline__ int swz_x(int row) { return row & 7; }
+__device__ __forceinline__ int swz_t8(int row) { return (row & 3) | ((row >> 3) & 1) << 4; }
 
 // FWD: the a operand passes act and leaves its checkpoint, bias is added.  Else (dgrad): out is
-// multiplied by act'.
-template <typename T, bool FWD, int ACT, int BN>
-__global__ void __launch_bounds__(kThreads) lin_nt_kernel(const NtArgs p) {
+// multiplied by act'.  VEC: rows of a and w are 16-byte aligned.
+template <typename T, bool FWD, int ACT, int BN, bool VEC>
+__global__ void __launch_bounds__(BN >= 256 ? 512 : 256) lin_nt_kernel(const NtArgs p) {
+  constexpr int NT = BN >= 256 ? 512 : 256;
   constexpr int BM = 128, PER = kPer16<T>, BK = 8 * PER;
-  constexpr int WN = BN / 64, WM = 4 / WN, TM = BM / WM / 16;  // a wave: TM * 16 rows x 64 columns
-  constexpr int XA = BM * 8 / kThreads, WB = BN * 8 / kThreads;
+  constexpr int WN = BN / 64, WM = NT / 64 / WN, TM = BM / WM / 16;  // a wave: TM * 16 rows x 64 columns
+  constexpr int XA = BM * 8 / NT, WB = BN * 8 / NT;
+  constexpr int RC = BN / PER;  // dgrad: chunks of a LDS row of w
   __shared__ uint4 xs[BM * 8];
   __shared__ uint4 ws[BN * 8];
 
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int wn = wid % WN, wm = wid / WN;
   const int g = lane >> 4, r = lane & 15;
-  // the column tiles of one row tile follow each other on one XCD: they share its L2's copy of A
+  // the column tiles of one row tile follow each other on one XCD: they share its L2's copy of a
   const int lb = mdev::xcd_logical(blockIdx.x, gridDim.x);
   const int nt = lb % p.ntiles;
   const int n0 = nt * BN;
   const int64_t m0 = static_cast<int64_t>(lb / p.ntiles) * BM;
-  const T* A = static_cast<const T*>(p.a);
-  const int chunk = tid & 7, srow = tid >> 3;  // staging: 32 rows a turn
+  const int chunk = tid & 7, srow = tid >> 3;  // staging of rows of 128 bytes
+  const bool wide = sizeof(T) == 2 && p.w_f32;
 
-  uint4 xr[XA], wr[WB], wr2[WB];
+  const __amdgpu_buffer_rsrc_t ar = range(static_cast<const T*>(p.a) + m0 * p.K,
+                                          (p.M - m0) * p.K * static_cast<int64_t>(sizeof(T)));
+  const int ew = wide ? 4 : static_cast<int>(sizeof(T));
+  const int64_t wskip = FWD ? static_cast<int64_t>(n0) * p.K : n0;
+  const __amdgpu_buffer_rsrc_t wr = range(static_cast<const char*>(p.w) + wskip * ew,
+                                          (static_cast<int64_t>(p.N) * p.K - wskip) * ew);
+
+  uint4 ra[XA], rw[WB], rw2[WB];
   auto fetch = [&](int k0) {
     const int k = k0 + chunk * PER;
 #pragma unroll
     for (int i = 0; i < XA; ++i) {
-      const int64_t m = m0 + srow + 32 * i;
-      xr[i] = load16<T>(A + m * p.K + k, m < p.M ? p.K - k : 0, p.va);
+      const uint32_t row = srow + NT / 8 * i;
+      ra[i] = load16<T, VEC>(ar, (row * p.K + k) * static_cast<uint32_t>(sizeof(T)), p.K - k);
     }
 #pragma unroll
     for (int i = 0; i < WB; ++i) {
-      const int n = n0 + srow + 32 * i;
-      const int have = n < p.N ? p.K - k : 0;
-      const int64_t off = static_cast<int64_t>(n) * p.K + k;
-      if (sizeof(T) == 2 && p.b_f32) {
-        wr[i] = load16<float>(static_cast<const float*>(p.b) + off, have, p.vb);
-        wr2[i] = load16<float>(static_cast<const float*>(p.b) + off + 4, have - 4, p.vb);
+      uint32_t off;
+      int have;
+      if constexpr (FWD) {
+        off = static_cast<uint32_t>(srow + NT / 8 * i) * p.K + k;
+        have = p.K - k;
       } else {
-        wr[i] = load16<T>(static_cast<const T*>(p.b) + off, have, p.vb);
+        const int id = tid + NT * i, row = id / RC, c = id % RC * PER;
+        off = static_cast<uint32_t>(k0 + row) * p.N + c;
+        have = k0 + row < p.K ? p.N - n0 - c : 0;
+      }
+      if (wide) {
+        rw[i] = load16<float, VEC>(wr, off * 4, have);
+        rw2[i] = load16<float, VEC>(wr, off * 4 + 16, have - 4);
+      } else {
+        rw[i] = load16<T, VEC>(wr, off * static_cast<uint32_t>(sizeof(T)), have);
       }
     }
   };
@@ -171,11 +231,11 @@ __global__ void __launch_bounds__(kThreads) lin_nt_kernel(const NtArgs p) {
     if (k0 > 0) __syncthreads();
 #pragma unroll
     for (int i = 0; i < XA; ++i) {
-      const int row = srow + 32 * i;
+      const int row = srow + NT / 8 * i;
       if constexpr (FWD) {
+        float v[PER];
+        if (ACT == kCkptGelu || (p.codes != nullptr && nt == 0)) unpack16<T>(ra[i], v);
         if (p.codes != nullptr && nt == 0) {
-          float v[PER];
-          unpack16<T>(xr[i], v);
           uint32_t m = 0;
 #pragma unroll
           for (int e = 0; e < PER; ++e) m = max(m, abs_bits(v[e]));
@@ -192,25 +252,34 @@ __global__ void __launch_bounds__(kThreads) lin_nt_kernel(const NtArgs p) {
           }
         }
         if constexpr (ACT == kCkptGelu) {
-          float v[PER];
-          unpack16<T>(xr[i], v);
 #pragma unroll
-          for (int e = 0; e < PER; ++e) v[e] = gelu(v[e]);
-          xr[i] = pack16<T>(v);
+          for (int e = 0; e < PER; ++e) v[e] = gelu<T>(v[e]);
+          ra[i] = pack16<T>(v);
         }
       }
-      xs[row * 8 + (chunk ^ swz_x(row))] = xr[i];
+      xs[row * 8 + (chunk ^ swz_a(row))] = ra[i];
     }
 #pragma unroll
     for (int i = 0; i < WB; ++i) {
-      const int row = srow + 32 * i;
-      if (sizeof(T) == 2 && p.b_f32) {
+      if (wide) {
         float v[8];
-        __builtin_memcpy(v, &wr[i], 16);
-        __builtin_memcpy(v + 4, &wr2[i], 16);
-        wr[i] = pack16<T>(v);
+        __builtin_memcpy(v, &rw[i], 16);
+        __builtin_memcpy(v + 4, &rw2[i], 16);
+        rw[i] = pack16<T>(v);
       }
-      ws[row * 8 + (chunk ^ swz_w(row))] = wr[i];
+      if constexpr (FWD) {
+        const int row = srow + NT / 8 * i;
+        ws[row * 8 + (chunk ^ swz_w(row))] = rw[i];
+      } else {
+        const int id = tid + NT * i, row = id / RC, c = id % RC;
+        if constexpr (sizeof(T) == 2) {
+          const int x = swz_t8(row);  // bit 0 of the unit: the two halves change places
+          const uint4 q = (x & 1) ? make_uint4(rw[i].z, rw[i].w, rw[i].x, rw[i].y) : rw[i];
+          ws[row * RC + (c ^ (x >> 1 & (RC - 1)))] = q;
+        } else {
+          ws[row * RC + c] = rw[i];
+        }
+      }
     }
     __syncthreads();
     if (k0 + BK < p.K) fetch(k0 + BK);
@@ -218,14 +287,39 @@ __global__ void __launch_bounds__(kThreads) lin_nt_kernel(const NtArgs p) {
     for (int s = 0; s < 2; ++s) {
       uint4 wf[4], xf[TM];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int row = wn * 64 + 16 * (r >> 2) + 4 * t + (r & 3);
-        wf[t] = ws[row * 8 + ((s * 4 + g) ^ swz_w(row))];
-      }
-#pragma unroll
       for (int t = 0; t < TM; ++t) {
         const int row = (wm * TM + t) * 16 + r;
-        xf[t] = xs[row * 8 + ((s * 4 + g) ^ swz_x(row))];
+        xf[t] = xs[row * 8 + ((s * 4 + g) ^ swz_a(row))];
+      }
+      if constexpr (FWD) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int row = wn * 64 + 16 * (r >> 2) + 4 * t + (r & 3);
+          wf[t] = ws[row * 8 + ((s * 4 + g) ^ swz_w(row))];
+        }
+      } else if constexpr (sizeof(T) == 2) {
+        // k = 8 g + 0..7: two reads of 4 rows; lane 4 q + c of the group supplies row q, columns 16 c + 4 t ..
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          uint2 h[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = s * 32 + g * 8 + 4 * e + (r >> 2);
+            const int unit = wn * 16 + (r & 3) * 4 + t;
+            h[e] = tr_read(reinterpret_cast<const uint2*>(ws) + row * (BN / 4) + (unit ^ (swz_t8(row) & (BN / 4 - 1))));
+          }
+          wf[t] = make_uint4(h[0].x, h[0].y, h[1].x, h[1].y);
+        }
+      } else {
+        // k = 4 g + i of this half: four columns a read, one for each tile
+        const float* base = reinterpret_cast<const float*>(ws) + wn * 64 + 4 * r;
+        float4 h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const float4*>(base + (s * 16 + 4 * g + i) * BN);
+        wf[0] = __builtin_bit_cast(uint4, make_float4(h[0].x, h[1].x, h[2].x, h[3].x));
+        wf[1] = __builtin_bit_cast(uint4, make_float4(h[0].y, h[1].y, h[2].y, h[3].y));
+        wf[2] = __builtin_bit_cast(uint4, make_float4(h[0].z, h[1].z, h[2].z, h[3].z));
+        wf[3] = __builtin_bit_cast(uint4, make_float4(h[0].w, h[1].w, h[2].w, h[3].w));
       }
 #pragma unroll
       for (int i = 0; i < TM; ++i)
@@ -244,8 +338,7 @@ __global__ void __launch_bounds__(kThreads) lin_nt_kernel(const NtArgs p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (nc + e < p.N)
-          bias[e] = (sizeof(T) == 2 && p.b_f32) ? static_cast<const float*>(p.bias)[nc + e]
-                                                 : Io<T>::ld(static_cast<const T*>(p.bias) + nc + e);
+          bias[e] = wide ? static_cast<const float*>(p.bias)[nc + e] : Io<T>::ld(static_cast<const T*>(p.bias) + nc + e);
     }
   }
 #pragma unroll
@@ -256,7 +349,7 @@ __global__ void __launch_bounds__(kThreads) lin_nt_kernel(const NtArgs p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * j + e] = acc[i][j][e];
+      for (int e = 0; e < 4; ++e) v[!FWD && sizeof(T) == 4 ? 4 * e + j : 4 * j + e] = acc[i][j][e];
     if constexpr (FWD) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) v[e] += bias[e];
@@ -270,7 +363,7 @@ __global__ void __launch_bounds__(kThreads) lin_nt_kernel(const NtArgs p) {
         float z[4];
         decode4(w4[j], sc, z);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * j + e] *= gelu_slope(z[e]);
+        for (int e = 0; e < 4; ++e) v[4 * j + e] *= gelu_slope<T>(z[e]);
       }
     }
     T* out = static_cast<T*>(p.out) + m * p.N + nc;
@@ -286,20 +379,6 @@ __global__ void __launch_bounds__(kThreads) lin_nt_kernel(const NtArgs p) {
   }
 }
 
-template <typename TW, typename T>
-__global__ void __launch_bounds__(256) lin_transpose_kernel(const TW* __restrict__ w, T* __restrict__ wt, int N, int K) {
-  __shared__ float t[32][33];
-  const int x = threadIdx.x & 31, y0 = threadIdx.x >> 5;
-  const int k0 = blockIdx.x * 32, n0 = blockIdx.y * 32;
-#pragma unroll
-  for (int y = y0; y < 32; y += 8)
-    if (n0 + y < N && k0 + x < K) t[y][x] = Io<TW>::ld(w + static_cast<int64_t>(n0 + y) * K + k0 + x);
-  __syncthreads();
-#pragma unroll
-  for (int y = y0; y < 32; y += 8)
-    if (k0 + y < K && n0 + x < N) Io<T>::st(wt + static_cast<int64_t>(k0 + y) * N + n0 + x, t[x][y]);
-}
-
 // ------------------------------------------------------------------------------- wgrad
 struct TnArgs {
   const void* dy;       // [M, N]
@@ -308,19 +387,14 @@ struct TnArgs {
   float* ws;            // [splits][N][K], then [splits][N] of db
   int64_t M, rows_per_split;
   int N, K, Cp, splits, ktiles, ntiles;
-  bool vy, want_db;
+  bool want_db;
 };
 
 // LDS rows of 128 (or 64) columns.  16 bits: the transposed reads of a 16-lane group take 4 rows x 32
 // bytes, the 4 groups rows 8 apart, so 32-byte units are XORed with (row & 3, row bit 3).
 __device__ __forceinline__ int swz_t(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
 
-__device__ __forceinline__ uint2 tr_read(const void* p) {
-  auto q = (__attribute__((address_space(3))) mdev::i16x4_t*)((__attribute__((address_space(3))) void*)const_cast<void*>(p));
-  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(q));
-}
-
-template <typename T, int ACT, int BT>  // BT x BT output tile, 2 x 2 waves
+template <typename T, int ACT, int BT, bool VEC>  // BT x BT output tile, 2 x 2 waves
 __global__ void __launch_bounds__(kThreads) lin_tn_kernel(const TnArgs p) {
   constexpr int PER = kPer16<T>;
   constexpr int BS = sizeof(T) == 2 ? 64 : 32;       // rows a step
@@ -342,28 +416,31 @@ __global__ void __launch_bounds__(kThreads) lin_tn_kernel(const TnArgs p) {
   const int k0 = kt * BT, n0 = tile / p.ktiles * BT;
   const int64_t mb = split * p.rows_per_split;
   const int64_t me = mb + p.rows_per_split < p.M ? mb + p.rows_per_split : p.M;
-  const T* Y = static_cast<const T*>(p.dy);
   const bool db = p.want_db && kt == 0;
+
+  const int64_t rows = me - mb;  // buffers over this split's rows: what lies behind reads 0
+  const __amdgpu_buffer_rsrc_t yb = range(static_cast<const T*>(p.dy) + mb * p.N, rows * p.N * static_cast<int64_t>(sizeof(T)));
+  const __amdgpu_buffer_rsrc_t cb = range(p.codes + mb * p.Cp, rows * p.Cp);
+  const __amdgpu_buffer_rsrc_t eb = range(p.scales + mb * (p.Cp / kBlock), rows * (p.Cp / kBlock));
 
   uint4 yr[YC], zr[ZC];
   uint8_t zb[ZC];
   auto fetch = [&](int64_t m1) {
+    const uint32_t mr = static_cast<uint32_t>(m1 - mb);
 #pragma unroll
     for (int i = 0; i < YC; ++i) {
       const int id = tid + i * kThreads;
-      const int64_t m = m1 + id / RC;
       const int n = n0 + (id % RC) * PER;
-      yr[i] = load16<T>(Y + m * p.N + n, m < me ? p.N - n : 0, p.vy);
+      yr[i] = load16<T, VEC>(yb, ((mr + id / RC) * p.N + n) * static_cast<uint32_t>(sizeof(T)), p.N - n);
     }
 #pragma unroll
     for (int i = 0; i < ZC; ++i) {
       const int id = tid + i * kThreads;
-      const int64_t m = m1 + id / CG;
       const int k = k0 + (id % CG) * 16;
-      const bool in = id < BS * CG && m < me && k < p.Cp;
-      const int64_t o = m * p.Cp + k;
-      zr[i] = in ? *reinterpret_cast<const uint4*>(p.codes + o) : make_uint4(0u, 0u, 0u, 0u);
-      zb[i] = in ? p.scales[o / kBlock] : 0;
+      const bool in = id < BS * CG && k < p.Cp;
+      const uint32_t o = (mr + id / CG) * p.Cp + k;
+      zr[i] = buf16(cb, in ? o : kOut);
+      zb[i] = static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(eb, static_cast<int>(in ? o / kBlock : kOut), 0, 0));
     }
   };
   auto at = [](int row, int chunk) {  // 16-byte slot of (row, chunk)
@@ -405,7 +482,7 @@ __global__ void __launch_bounds__(kThreads) lin_tn_kernel(const TnArgs p) {
         for (int q = 0; q < 4; ++q) decode4(w4[q], sc, v + 4 * q);
         if constexpr (ACT == kCkptGelu) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = gelu(v[e]);
+          for (int e = 0; e < 16; ++e) v[e] = gelu<T>(v[e]);
         }
 #pragma unroll
         for (int e = 0; e < 16; e += PER) zs[at(id / CG, (id % CG) * (16 / PER) + e / PER)] = pack16<T>(v + e);
@@ -550,13 +627,19 @@ WgradPlan wgrad_plan(int64_t M, int N, int K) {
   return w;
 }
 
-template <typename T, bool FWD, int ACT>
-void launch_nt(NtArgs p, hipStream_t st) {
-  const int bn = p.N <= 64 ? 64 : 128;
-  p.ntiles = (p.N + bn - 1) / bn;
+template <typename T, bool FWD, int ACT, int BN>
+void launch_nt_bn(NtArgs p, bool vec, hipStream_t st) {
+  p.ntiles = (p.N + BN - 1) / BN;
   const unsigned grid = static_cast<unsigned>((p.M + 127) / 128 * p.ntiles);
-  if (bn == 64) lin_nt_kernel<T, FWD, ACT, 64><<<grid, kThreads, 0, st>>>(p);
-  else lin_nt_kernel<T, FWD, ACT, 128><<<grid, kThreads, 0, st>>>(p);
+  constexpr int threads = BN >= 256 ? 512 : 256;
+  if (vec) lin_nt_kernel<T, FWD, ACT, BN, true><<<grid, threads, 0, st>>>(p);
+  else lin_nt_kernel<T, FWD, ACT, BN, false><<<grid, threads, 0, st>>>(p);
+}
+template <typename T, bool FWD, int ACT>
+void launch_nt(const NtArgs& p, bool vec, hipStream_t st) {
+  if (p.N <= 64) launch_nt_bn<T, FWD, ACT, 64>(p, vec, st);
+  else if (p.N <= 128) launch_nt_bn<T, FWD, ACT, 128>(p, vec, st);
+  else launch_nt_bn<T, FWD, ACT, 256>(p, vec, st);
 }
 
 }  // namespace
@@ -564,42 +647,31 @@ void launch_nt(NtArgs p, hipStream_t st) {
 void launch_lin_fwd(const LinFwdArgs& a, hipStream_t st) {
   if (a.M == 0) return;
   NtArgs p{};
-  p.a = a.x; p.b = a.w; p.bias = a.b; p.out = a.y; p.codes = a.codes; p.scales = a.scales;
+  p.a = a.x; p.w = a.w; p.bias = a.b; p.out = a.y; p.codes = a.codes; p.scales = a.scales;
   p.M = a.M; p.N = a.N; p.K = a.K; p.Cp = static_cast<int>(padded(a.K));
   const int per = 16 / elem(a.dtype);
-  p.b_f32 = a.w_dtype == kF32;
-  p.va = a.K % per == 0 && al16(a.x);
-  p.vb = a.K % (p.b_f32 && a.dtype != kF32 ? 8 : per) == 0 && al16(a.w);
+  p.w_f32 = a.w_dtype == kF32;
   p.vo = a.N % per == 0 && al16(a.y);
+  const bool vec = a.K % per == 0 && al16(a.x) && al16(a.w);
   by_type(a.dtype, [&](auto t) {
-    if (a.act == kCkptGelu) launch_nt<decltype(t), true, kCkptGelu>(p, st);
-    else launch_nt<decltype(t), true, kCkptNone>(p, st);
-  });
-}
-
-void launch_lin_transpose(const void* w, int w_dtype, void* wt, int dtype, int N, int K, hipStream_t st) {
-  const dim3 grid((K + 31) / 32, (N + 31) / 32);
-  by_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    if (w_dtype == kF32) lin_transpose_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(w), static_cast<T*>(wt), N, K);
-    else lin_transpose_kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(w), static_cast<T*>(wt), N, K);
+    if (a.act == kCkptGelu) launch_nt<decltype(t), true, kCkptGelu>(p, vec, st);
+    else launch_nt<decltype(t), true, kCkptNone>(p, vec, st);
   });
 }
 
 void launch_lin_dgrad(const LinDgradArgs& a, hipStream_t st) {
   if (a.M == 0) return;
   NtArgs p{};
-  p.a = a.dy; p.b = a.wt; p.out = a.dx;
+  p.a = a.dy; p.w = a.w; p.out = a.dx;
   p.codes = const_cast<int8_t*>(a.codes); p.scales = const_cast<uint8_t*>(a.scales);
   p.M = a.M; p.N = a.K; p.K = a.N; p.Cp = static_cast<int>(padded(a.K));
   const int per = 16 / elem(a.dtype);
-  p.b_f32 = false;
-  p.va = a.N % per == 0 && al16(a.dy);
-  p.vb = a.N % per == 0 && al16(a.wt);
+  p.w_f32 = a.w_dtype == kF32;
   p.vo = a.K % per == 0 && al16(a.dx);
+  const bool vec = a.N % per == 0 && a.K % per == 0 && al16(a.dy) && al16(a.w);
   by_type(a.dtype, [&](auto t) {
-    if (a.act == kCkptGelu) launch_nt<decltype(t), false, kCkptGelu>(p, st);
-    else launch_nt<decltype(t), false, kCkptNone>(p, st);
+    if (a.act == kCkptGelu) launch_nt<decltype(t), false, kCkptGelu>(p, vec, st);
+    else launch_nt<decltype(t), false, kCkptNone>(p, vec, st);
   });
 }
 
@@ -614,19 +686,21 @@ void launch_lin_wgrad(const LinWgradArgs& a, hipStream_t st) {
   p.dy = a.dy; p.codes = a.codes; p.scales = a.scales; p.ws = a.ws;
   p.M = a.M; p.rows_per_split = w.rows; p.N = a.N; p.K = a.K; p.Cp = static_cast<int>(padded(a.K));
   p.splits = w.splits;
-  p.vy = a.N % (16 / elem(a.dtype)) == 0 && al16(a.dy);
+  const bool vec = a.N % (16 / elem(a.dtype)) == 0 && al16(a.dy);
   p.want_db = a.db != nullptr;
   p.ktiles = (a.K + w.tile - 1) / w.tile;
   p.ntiles = (a.N + w.tile - 1) / w.tile;
   const unsigned grid = static_cast<unsigned>(p.ktiles * p.ntiles * w.splits);
   by_type(a.dtype, [&](auto t) {
     using T = decltype(t);
+    auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, st>>>(p); };
+    const bool gelu = a.act == kCkptGelu;
     if (w.tile == 64) {
-      if (a.act == kCkptGelu) lin_tn_kernel<T, kCkptGelu, 64><<<grid, kThreads, 0, st>>>(p);
-      else lin_tn_kernel<T, kCkptNone, 64><<<grid, kThreads, 0, st>>>(p);
+      if (vec) go(gelu ? lin_tn_kernel<T, kCkptGelu, 64, true> : lin_tn_kernel<T, kCkptNone, 64, true>);
+      else go(gelu ? lin_tn_kernel<T, kCkptGelu, 64, false> : lin_tn_kernel<T, kCkptNone, 64, false>);
     } else {
-      if (a.act == kCkptGelu) lin_tn_kernel<T, kCkptGelu, 128><<<grid, kThreads, 0, st>>>(p);
-      else lin_tn_kernel<T, kCkptNone, 128><<<grid, kThreads, 0, st>>>(p);
+      if (vec) go(gelu ? lin_tn_kernel<T, kCkptGelu, 128, true> : lin_tn_kernel<T, kCkptNone, 128, true>);
+      else go(gelu ? lin_tn_kernel<T, kCkptGelu, 128, false> : lin_tn_kernel<T, kCkptNone, 128, false>);
     }
   });
   const int64_t plane = static_cast<int64_t>(a.N) * a.K;

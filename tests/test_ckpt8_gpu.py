@@ -184,6 +184,17 @@ def test_linear_far_gelu_inputs():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_gelu_of_infinity_and_nan(dtype):
+    x = torch.zeros(3, 32, device="cuda", dtype=dtype)
+    x[0, 0], x[1, 0] = float("inf"), float("nan")
+    w = torch.zeros(32, 32, device="cuda", dtype=dtype)
+    w[0, 0] = 1.0
+    y = ops.linear_ckpt8(x, w, None, act="gelu")
+    # 0 * inf in the other columns of the row, as in any product
+    assert y[0, 0] == float("inf") and torch.isnan(y[1, 0]) and not y[2].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_bits_are_the_same_on_every_run_and_stream(dtype):
     x, w = _rand(9000, 160, dtype=dtype).requires_grad_(True), _rand(200, 160, seed=1, dtype=dtype).requires_grad_(True)
     b, dy = _rand(200, seed=2, dtype=dtype).requires_grad_(True), _rand(9000, 200, seed=3, dtype=dtype)
