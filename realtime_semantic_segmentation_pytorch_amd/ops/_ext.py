@@ -9,6 +9,7 @@ Policy (see README "Kernel dispatch"):
 """
 from __future__ import annotations
 
+import functools
 import os
 import threading
 
@@ -90,6 +91,23 @@ def use_hip(t: torch.Tensor, family: str | None = None) -> bool:
             "rtseg HIP extension is required for GPU tensors but failed to load: "
             f"{_load_error!r}. Build it with `python -m realtime_semantic_segmentation_pytorch_amd.ops.build`.")
     return True
+
+
+def differentiable_once(backward):
+    """For the backward of a ``torch.autograd.Function``: its gradients have no graph of their own, so under
+    ``create_graph`` any further use of them raises instead of passing for a constant."""
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        err = torch._C._functions.DelayedError(
+            b"rtseg: this gradient cannot be differentiated again (the operator is differentiable once)", len(out))
+        return err(*[None if g is None else g.detach().requires_grad_() for g in out])
+
+    return run
 
 
 class _TracedOps:

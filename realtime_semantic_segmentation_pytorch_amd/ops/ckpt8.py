@@ -30,9 +30,8 @@ from typing import NamedTuple, Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
-from ._ext import ops, use_hip
+from ._ext import differentiable_once, ops, use_hip
 
 BLOCK = 32
 ACTS = {"none": 0, "gelu": 1}
@@ -144,34 +143,23 @@ def linear_ckpt8_reference(x2, weight, bias, act):
 
 
 class _LinearCkpt8Fn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x2, weight, bias, act, hip):
-        need_x, need_w = ctx.needs_input_grad[:2]
-        keep = need_w or (need_x and act != "none")
-        if hip:
-            y, codes, scales = ops().linear_ckpt8_fwd(x2, weight, bias, ACTS[act], keep)
-        else:
-            y = linear_ckpt8_reference(x2, weight, bias, act)
-            codes, scales = _pack_reference(x2) if keep else (None, None)
-        ctx.act, ctx.hip, ctx.k, ctx.wtype = act, hip, x2.shape[1], weight.dtype
-        ctx.save_for_backward(codes if keep else None, scales if keep else None, weight if need_x else None)
-        return y
+    """The PyTorch formulation (CPU tensors)."""
 
     @staticmethod
-    @once_differentiable
+    def forward(ctx, x2, weight, bias, act):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        keep = need_w or (need_x and act != "none")
+        codes, scales = _pack_reference(x2) if keep else (None, None)
+        ctx.act, ctx.k, ctx.wtype = act, x2.shape[1], weight.dtype
+        ctx.save_for_backward(codes, scales, weight if need_x else None)
+        return linear_ckpt8_reference(x2, weight, bias, act)
+
+    @staticmethod
+    @differentiable_once
     def backward(ctx, dy):
         codes, scales, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dy = dy.contiguous()
         dx = dw = db = None
-        if ctx.hip:
-            if need_x:
-                dx = ops().linear_ckpt8_dgrad(dy, weight, codes, scales, ACTS[ctx.act])
-            if need_w:
-                dw, db = ops().linear_ckpt8_wgrad(dy, codes, scales, ctx.k, ACTS[ctx.act], ctx.wtype, need_b)
-            elif need_b:
-                db = ops().linear_ckpt8_bgrad(dy, ctx.wtype)
-            return dx, dw, db, None, None
         z = None if codes is None else _unpack_reference(codes, scales, ctx.k, torch.float32)
         g = dy.float()
         if need_x:
@@ -182,7 +170,7 @@ class _LinearCkpt8Fn(torch.autograd.Function):
             dw = (g.t() @ a).to(ctx.wtype)
         if need_b:
             db = g.sum(0).to(ctx.wtype)
-        return dx, dw, db, None, None
+        return dx, dw, db, None
 
 
 def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -213,9 +201,11 @@ def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     for p in (weight, bias):
         if p is not None and p.device != x.device:
             raise ValueError(f"linear_ckpt8: all tensors must be on one device, got {x.device} and {p.device}")
-    x2 = _rows(x, "linear_ckpt8")
-    b = None if bias is None else bias.contiguous()
-    y = _LinearCkpt8Fn.apply(x2, weight.contiguous(), b, act, use_hip(x2, "ckpt8"))
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"linear_ckpt8: fp32, bf16 or fp16 expected, got {x.dtype}")
+    if use_hip(x, "ckpt8"):
+        return ops().linear_ckpt8(x, weight, bias, ACTS[act])
+    y = _LinearCkpt8Fn.apply(_rows(x, "linear_ckpt8"), weight, bias, act)
     return y.view(*x.shape[:-1], weight.shape[0])
 
 

@@ -18,9 +18,8 @@ from typing import Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
-from ._ext import ops, use_hip
+from ._ext import differentiable_once, ops, use_hip
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _MAX_CHANNELS = 8192  # a row is held in one block's registers
@@ -47,54 +46,6 @@ def layer_norm_reference(x, weight=None, bias=None, eps=1e-5, residual=None, out
     return y if residual is None else (s, y)
 
 
-class _LayerNormFn(torch.autograd.Function):
-    """(x, residual | None) -> y, or (x + residual, y)."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps, out_dtype, ckpt8, want_sum):
-        shape, c = x.shape, x.shape[-1]
-        x2 = x.reshape(-1, c).contiguous()
-        r2 = None if residual is None else residual.reshape(-1, c).contiguous()
-        w = None if weight is None else weight.detach().float().contiguous()
-        b = None if bias is None else bias.detach().float().contiguous()
-        train = any(ctx.needs_input_grad)
-        keep = (2 if ckpt8 else 1) if train else 0
-        # without a checkpoint the backward normalises the sum again, so it is kept even if unwanted
-        s, y, mean, rstd, codes, scales = ops().layer_norm_fwd(x2, r2, w, b, eps, out_dtype, keep,
-                                                               want_sum or keep == 1)
-        ctx.set_materialize_grads(False)
-        if train:
-            ctx.shape, ctx.types = shape, (x.dtype, None if residual is None else residual.dtype)
-            ctx.param_types = (weight.dtype if weight is not None else None, bias.dtype if bias is not None else None)
-            kept = (codes, scales) if ckpt8 else (x2 if residual is None else s, None)
-            ctx.save_for_backward(*kept, mean, rstd, w)
-        y = y.view(shape)
-        return (s.view(shape) if want_sum else None), y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, ds, dy):
-        first, scales, mean, rstd, w = ctx.saved_tensors
-        shape, (xt, rt) = ctx.shape, ctx.types
-        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
-        if dy is None:  # the norm's output is unused: only the sum carries a gradient
-            gx = ds if need_x else None
-            gr = ds.to(rt) if (need_r and ds is not None) else None
-            return gx, gr, None, None, None, None, None, None
-        c = shape[-1]
-        dy = dy.reshape(-1, c).contiguous()
-        ds = None if ds is None else ds.reshape(-1, c).contiguous()
-        x, codes = (first, None) if scales is None else (None, first)
-        own_r = need_r and rt != xt
-        dx, dr, dw, db = ops().layer_norm_bwd(dy, ds, x, codes, scales, mean, rstd, w, xt, rt,
-                                              need_x or (need_r and not own_r), own_r, need_w or need_b)
-        dx = None if dx is None else dx.view(shape)
-        gr = None if not need_r else (dr.view(shape) if own_r else dx)
-        wt, bt = ctx.param_types
-        return (dx if need_x else None, gr, dw.to(wt) if need_w else None, db.to(bt) if need_b else None,
-                None, None, None, None)
-
-
 class _LayerNormCkptFn(torch.autograd.Function):
     """The PyTorch formulation with an 8-bit checkpoint (CPU tensors)."""
 
@@ -117,7 +68,7 @@ class _LayerNormCkptFn(torch.autograd.Function):
         return h.to(out_dtype)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, dy):
         from .ckpt8 import ckpt8_unpack
 
@@ -166,9 +117,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if x.dtype in _DTYPES and out_dtype in _DTYPES and c <= _MAX_CHANNELS and use_hip(x, "layer_norm"):
         # 16 bits in and another 16-bit type out: through fp32
         got = out_dtype if out_dtype == x.dtype or torch.float32 in (out_dtype, x.dtype) else torch.float32
-        s, y = _LayerNormFn.apply(x, residual, weight, bias, float(eps), got, bool(ckpt8), residual is not None and want_sum)
+        *s, y = ops().layer_norm(x, residual, weight, bias, eps, got, ckpt8, residual is not None and want_sum)
         y = y if got == out_dtype else y.to(out_dtype)
-        return y if residual is None else (s, y)
+        return y if residual is None else (s[0] if s else None, y)
     if ckpt8 and x.dtype in _DTYPES and torch.is_grad_enabled():
         s = x if residual is None else x + residual
         y = _LayerNormCkptFn.apply(s, weight, bias, float(eps), out_dtype)

@@ -214,8 +214,8 @@ def test_linear_refusals():
         ops.ckpt8_unpack(ops.ckpt8_pack(x), torch.int8)
     y = ops.linear_ckpt8(x.requires_grad_(True), w.requires_grad_(True), None)
     (g,) = torch.autograd.grad(y.sum(), w, create_graph=True)
-    with pytest.raises(RuntimeError):
-        g.sum().backward()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (g * w).sum().backward()
 
 
 # ------------------------------------------------------------------------------- layer norm

@@ -168,6 +168,22 @@ def test_linear_non_finite_inputs_show_in_the_gradients(dtype):
     assert torch.isfinite(x.grad).all()
 
 
+def test_linear_takes_the_hip_path_and_refuses():
+    x, w = _rand(8, 32).requires_grad_(True), _rand(4, 32, seed=1).requires_grad_(True)
+    y = ops.linear_ckpt8(x, w)
+    assert "LinearCkpt8Fn" in y.grad_fn.name()
+    (g,) = torch.autograd.grad(y.sum(), w, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (g * w).sum().backward()
+    with pytest.raises(ValueError, match="one device"):
+        ops.linear_ckpt8(x, w.detach().cpu())
+    y = ops.linear_ckpt8(x, w)
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_linear_far_gelu_inputs():
     """The activation's tails: 0 and the identity, without a NaN from 0 * inf."""
     x = torch.tensor([[-300.0, -40.0, -9.0, -6.0, -3.0, 0.0, 3.0, 6.0, 9.0, 40.0, 300.0, 1e4]] * 3)
