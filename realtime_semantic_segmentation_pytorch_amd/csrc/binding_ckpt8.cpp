@@ -224,14 +224,11 @@ int act_code(int64_t act) {
 std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ckpt8_fwd(const at::Tensor& x, const at::Tensor& w,
                                                                 const std::optional<at::Tensor>& b, int64_t act, bool keep) {
   check_rows(x, "linear_ckpt8", "x");
-  TORCH_CHECK(w.dim() == 2 && w.size(0) >= 1 && w.size(0) <= kMaxChannels,
-              "rtseg.linear_ckpt8: weight must be [out, in] with 1 .. ", kMaxChannels, " outputs");
+  TORCH_CHECK(w.dim() == 2 && w.size(0) >= 1 && w.size(0) <= kMaxChannels && w.scalar_type() == x.scalar_type(),
+              "rtseg.linear_ckpt8: weight must be [out, in] of x's type with 1 .. ", kMaxChannels, " outputs");
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   check_param(w, {N, K}, x, "linear_ckpt8", "weight");
-  if (b.has_value()) {
-    check_param(*b, {N}, x, "linear_ckpt8", "bias");
-    TORCH_CHECK(b->scalar_type() == w.scalar_type(), "rtseg.linear_ckpt8: weight and bias must be of one type");
-  }
+  if (b.has_value()) check_param(*b, {N}, x, "linear_ckpt8", "bias");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   at::Tensor y = at::empty({M, N}, x.options()), codes, scales;
   LinFwdArgs a{};
@@ -245,7 +242,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ckpt8_fwd(const at::Tensor
   a.b = opt_ptr(b);
   a.y = y.data_ptr();
   a.dtype = dtype_code(x);
-  a.w_dtype = dtype_code(w);
+  a.b_dtype = b.has_value() ? dtype_code(*b) : a.dtype;
   a.act = act_code(act);
   a.M = M;
   a.N = static_cast<int>(N);
@@ -261,6 +258,7 @@ at::Tensor linear_ckpt8_dgrad(const at::Tensor& dy, const at::Tensor& w, const s
               "rtseg.linear_ckpt8_dgrad: weight must be [out, in]");
   const int64_t M = dy.size(0), N = dy.size(1), K = w.size(1);
   check_param(w, {N, K}, dy, "linear_ckpt8_dgrad", "weight");
+  TORCH_CHECK(w.scalar_type() == dy.scalar_type(), "rtseg.linear_ckpt8_dgrad: the weight must be of the gradient's type");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dy.device());
   at::Tensor dx = at::empty({M, K}, dy.options());
   LinDgradArgs a{};
@@ -274,7 +272,6 @@ at::Tensor linear_ckpt8_dgrad(const at::Tensor& dy, const at::Tensor& w, const s
   if (M == 0) return dx;
   a.dy = dy.data_ptr();
   a.w = w.data_ptr();
-  a.w_dtype = dtype_code(w);
   a.dx = dx.data_ptr();
   a.dtype = dtype_code(dy);
   a.M = M;
@@ -307,7 +304,7 @@ std::tuple<at::Tensor, at::Tensor> linear_ckpt8_wgrad(const at::Tensor& dy, cons
   a.M = M;
   a.N = static_cast<int>(N);
   a.K = static_cast<int>(K);
-  at::Tensor ws = at::empty({lin_wgrad_ws_elems(M, a.N, a.K)}, dy.options().dtype(at::kFloat));
+  at::Tensor ws = at::empty({lin_wgrad_ws_elems(M, a.N, a.K, a.act)}, dy.options().dtype(at::kFloat));
   a.ws = ws.data_ptr<float>();
   launch_lin_wgrad(a, cur_stream());
   return {dw, db};
@@ -350,7 +347,8 @@ std::optional<at::Tensor> maybe(const at::Tensor& t) { return t.defined() ? std:
 struct LinearCkpt8Fn : torch::autograd::Function<LinearCkpt8Fn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
                             const std::optional<at::Tensor>& b, int64_t act, bool need_x, bool need_w, bool need_b) {
-    const at::Tensor x2 = rows_of(x), wc = w.contiguous();
+    // fp32 weights beside 16-bit operands are cast once, for the forward and the data gradient
+    const at::Tensor x2 = rows_of(x), wc = w.to(x.scalar_type()).contiguous();
     auto [y, codes, scales] = linear_ckpt8_fwd(x2, wc, b, act, need_w || (need_x && act != kCkptNone));
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({codes, scales, need_x ? wc : at::Tensor()});
@@ -382,7 +380,7 @@ at::Tensor linear_ckpt8(const at::Tensor& x, const at::Tensor& w, const std::opt
   const at::Tensor x2 = rows_of(x);
   auto shape = x.sizes().vec();
   shape.back() = w.size(0);
-  return std::get<0>(linear_ckpt8_fwd(x2, w.contiguous(), b, act, false)).view(shape);
+  return std::get<0>(linear_ckpt8_fwd(x2, w.to(x.scalar_type()).contiguous(), b, act, false)).view(shape);
 }
 at::Tensor linear_ckpt8_autograd(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& b, int64_t act) {
   const bool on = at::GradMode::is_enabled();

@@ -490,16 +490,16 @@ void launch_layer_norm_bwd(LnBwdArgs a, float* dw, float* db, hipStream_t st);
 
 // ---- linear_ckpt8.hip ---------------------------------------------------------------
 // y = act(x) w^T + b for x [M, K], w [N, K]; the checkpoint of x is written by the forward and read by
-// both gradients.  x / y / dy / dx are of one type (fp32 / bf16 / fp16); w and b that type or fp32.
+// both gradients.  x / y / dy / dx / w are of one type (fp32 / bf16 / fp16); b that type or fp32.
 enum CkptAct : int { kCkptNone = 0, kCkptGelu = 1 };
 struct LinFwdArgs {
   const void* x;
   const void* w;
-  const void* b;      // [N] of w's type, or nullptr
+  const void* b;      // [N] or nullptr
   void* y;
   int8_t* codes;      // or nullptr: nothing is kept
   uint8_t* scales;
-  int dtype, w_dtype, act;
+  int dtype, b_dtype, act;
   int64_t M;
   int N, K;
 };
@@ -509,7 +509,7 @@ struct LinDgradArgs {
   const int8_t* codes;  // read with act != none only
   const uint8_t* scales;
   void* dx;           // [M, K]
-  int dtype, w_dtype, act;
+  int dtype, act;
   int64_t M;
   int N, K;
 };
@@ -517,16 +517,16 @@ struct LinWgradArgs {
   const void* dy;
   const int8_t* codes;
   const uint8_t* scales;
-  float* ws;          // lin_wgrad_ws_elems
-  void* dw;           // [N, K], or nullptr
-  void* db;           // [N], or nullptr
-  int dtype, w_dtype, act;
+  float* ws;          // lin_wgrad_ws_elems floats
+  void* dw;           // [N, K] of w_dtype
+  void* db;           // [N] of w_dtype, or nullptr
+  int dtype, w_dtype, act;  // w_dtype: dtype or fp32
   int64_t M;
   int N, K;
 };
 void launch_lin_fwd(const LinFwdArgs& a, hipStream_t st);
 void launch_lin_dgrad(const LinDgradArgs& a, hipStream_t st);
-int64_t lin_wgrad_ws_elems(int64_t M, int N, int K);
+int64_t lin_wgrad_ws_elems(int64_t M, int N, int K, int act);
 void launch_lin_wgrad(const LinWgradArgs& a, hipStream_t st);
 // db [N] = column sums of dy [M, N]; ws: lin_colsum_splits(M) * N floats
 int lin_colsum_splits(int64_t M);

@@ -1,0 +1,193 @@
+// Device helpers of the checkpointing linear layer's kernels (linear_ckpt8_*.hip): activation, operand
+// loads and conversions, matrix instructions, LDS layouts.
+//
+//   forward   y = act(x) w^T + b          codes = checkpoint of x (rtseg_ckpt8.h)
+//   dgrad     dx = (dy w) * act'(z)       z = the checkpoint's values
+//   wgrad     dw = dy^T act(z), db = sum_rows dy
+//
+// bf16 / fp16 operands feed v_mfma_f32_16x16x32, fp32 ones v_mfma_f32_16x16x4_f32; sums are fp32.
+// act = gelu is computed in fp32 and rounded to the operands' type in front of the product, which is
+// what a separate activation layer hands to a linear layer.
+#pragma once
+
+#include "rtseg_ckpt8.h"
+#include "rtseg_launch.h"
+#include "rtseg_mfma_dev.h"
+
+namespace rtseg {
+namespace lin {
+
+using namespace ckpt8;
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+
+// Phi(-a), the normal tail, for a >= 0: log2 Phi(-a) is smooth, and a polynomial of degree 7 (minimax over
+// [0, 9], the error weighted by Phi and, up to a = 6.5, by itself; -inf beyond) gives Phi within 3e-7, and
+// within 2^-11.8 of its own value where it is small.
+__device__ __forceinline__ float normal_tail(float a) {
+  float q = __builtin_fmaf(a, -7.709749070272665e-07f, 4.193515997030772e-05f);
+  q = __builtin_fmaf(a, q, -0.0007947825361043215f);
+  q = __builtin_fmaf(a, q, 0.008072120137512684f);
+  q = __builtin_fmaf(a, q, -0.05329299345612526f);
+  q = __builtin_fmaf(a, q, -0.4589170515537262f);
+  q = __builtin_fmaf(a, q, -1.151143193244934f);
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(a, q, -0.9999992251396179f));
+}
+// gelu(x) = x Phi(x) = max(x, 0) - |x| Phi(-|x|), gelu'(x) = Phi(x) + x phi(x).  16-bit operands take the tail
+// above (10 full-rate instructions and one quarter-rate; erff costs five times that, and the activation is
+// what bounds the wide layers' forward); fp32 ones erff.
+template <typename T>
+__device__ __forceinline__ float gelu(float x) {
+  if constexpr (sizeof(T) == 4) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+  const float ax = fabsf(x);  // the factor is cut off where the tail is 0: inf - inf * 0 is inf
+  return __builtin_fmaf(-fminf(ax, 64.f), normal_tail(ax), fmaxf(x, 0.f));
+}
+template <typename T>
+__device__ __forceinline__ float gelu_slope(float x) {
+  if constexpr (sizeof(T) == 4)
+    return 0.5f * (1.f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * __expf(-0.5f * x * x);
+  const float e = __builtin_amdgcn_exp2f(x * x * -0.72134752044448170f), tail = normal_tail(fabsf(x));
+  return __builtin_fmaf(x * 0.39894228040143268f, e, x >= 0.f ? 1.f - tail : tail);
+}
+
+// 16 bytes of operand: 8 (bf16 / fp16) or 4 (fp32) consecutive k
+template <typename T> constexpr int kPer16 = 16 / static_cast<int>(sizeof(T));
+
+template <typename T>
+__device__ __forceinline__ void unpack16(uint4 q, float* v) {
+  T t[kPer16<T>];
+  __builtin_memcpy(t, &q, 16);
+#pragma unroll
+  for (int i = 0; i < kPer16<T>; ++i) v[i] = Io<T>::ld(t + i);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float* v) {
+  T t[kPer16<T>];
+#pragma unroll
+  for (int i = 0; i < kPer16<T>; ++i) Io<T>::st(t + i, v[i]);
+  uint4 q;
+  __builtin_memcpy(&q, t, 16);
+  return q;
+}
+template <>
+__device__ __forceinline__ uint4 pack16<uint16_t>(const float* v) {
+  return make_uint4(f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]),
+                    f32x2_to_bf16x2(v[6], v[7]));
+}
+
+// A range of a tensor as a buffer: loads past `bytes` read 0 and stores there are dropped, so the rows
+// that a tile does not have cost no branch.  kOut as an offset is past every range.
+constexpr uint32_t kOut = 0xfffffff0u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t range(const void* p, int64_t bytes) {
+  const uint32_t n = bytes < 0 ? 0u : bytes > 0xffffff00ll ? 0xffffff00u : static_cast<uint32_t>(bytes);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(n), 0x00020000);
+}
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+// `off` alone decides whether an access is in range; `base` (uniform, added to it) only moves along a row,
+// between columns that the caller has checked, so that a range has to end at the last row and no sooner
+__device__ __forceinline__ uint4 buf16(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t base = 0) {
+  return __builtin_bit_cast(
+      uint4, static_cast<u32x4_t>(__builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(off), static_cast<int>(base), 0)));
+}
+__device__ __forceinline__ uint8_t buf1(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t base = 0) {
+  return static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(r, static_cast<int>(off), static_cast<int>(base), 0));
+}
+__device__ __forceinline__ void put16(__amdgpu_buffer_rsrc_t r, uint32_t off, uint4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), r, static_cast<int>(off), 0, 0);
+}
+__device__ __forceinline__ void put8(__amdgpu_buffer_rsrc_t r, uint32_t off, uint2 v) {
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, v), r, static_cast<int>(off), 0, 0);
+}
+// four values of a 16-bit T
+template <typename T>
+__device__ __forceinline__ uint2 pack8(const float* v) {
+  if constexpr (__is_same(T, _Float16)) {
+    const _Float16 t[4] = {static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]),
+                           static_cast<_Float16>(v[3])};
+    return __builtin_bit_cast(uint2, t);
+  } else {
+    return make_uint2(f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]));
+  }
+}
+
+// Rows of any alignment.  The load is issued without a branch, from inside the tensor: p[i] where 16 bytes
+// fit behind it, else from its last 16 bytes (the tensor has at least that many where a row does; rows that
+// are shorter are left to settle16).  A value for which fewer than 16 bytes exist is settled when it is
+// used, after the wait: 0 where nothing exists, a row's last elements one by one.
+template <typename T>
+__device__ __forceinline__ uint4 any16(const T* p, int64_t i, int64_t size) {
+  uint4 q = make_uint4(0u, 0u, 0u, 0u);
+  const int64_t last = size - kPer16<T>;
+  if (last >= 0) __builtin_memcpy(&q, p + (i < last ? i : last), 16);
+  return q;
+}
+template <typename T>
+__device__ __forceinline__ uint4 settle16(uint4 q, const T* p, int64_t i, int n) {
+  if (n <= 0) return make_uint4(0u, 0u, 0u, 0u);
+  if (n < kPer16<T>) {
+    T t[kPer16<T>];
+#pragma unroll
+    for (int e = 0; e < kPer16<T>; ++e) {
+      t[e] = T(0);
+      if (e < n) t[e] = p[i + e];
+    }
+    __builtin_memcpy(&q, t, 16);
+  }
+  return q;
+}
+
+// largest of the chunk's absolute values as the bits of an fp32, NaN above infinity above every number
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(uint4 q, const float* v) {
+  if constexpr (sizeof(T) == 4) {
+    return max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+  } else {
+    typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+    auto half = [](uint32_t w) { return __builtin_bit_cast(u16x2_t, w & 0x7fff7fffu); };
+    const u16x2_t m = __builtin_elementwise_max(__builtin_elementwise_max(half(q.x), half(q.y)),
+                                                __builtin_elementwise_max(half(q.z), half(q.w)));
+    const unsigned short top = m.x > m.y ? m.x : m.y;
+    if constexpr (__is_same(T, _Float16)) return __float_as_uint(static_cast<float>(__builtin_bit_cast(_Float16, top)));
+    else return static_cast<uint32_t>(top) << 16;
+  }
+}
+
+// one 16x16 tile step over 64 bytes of k a row: lane (g = lane / 16) holds k = g * kPer16 .. + kPer16 - 1
+// of its row, for A and B alike
+template <typename T>
+__device__ __forceinline__ f32x4_t mma16(uint4 a, uint4 b, f32x4_t c) {
+  if constexpr (sizeof(T) == 4) {
+    float x[4], y[4];
+    __builtin_memcpy(x, &a, 16);
+    __builtin_memcpy(y, &b, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+    return c;
+  } else if constexpr (__is_same(T, _Float16)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(mdev::as_frag(a), mdev::as_frag(b), c, 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ uint2 tr_read(const void* p) {
+  auto q = (__attribute__((address_space(3))) mdev::i16x4_t*)((__attribute__((address_space(3))) void*)const_cast<void*>(p));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(q));
+}
+
+// LDS rows of an operand whose sum runs along them: 8 chunks of 16 bytes, chunk ^ (row & 7), which spreads
+// the 16 rows of a fragment read over the banks
+__device__ __forceinline__ int swz_a(int row) { return row & 7; }
+
+inline bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+inline int elem(int dt) { return dt == kF32 ? 4 : 2; }
+template <class F>
+void by_type(int dt, F f) {
+  if (dt == kF32) f(float{});
+  else if (dt == kBF16) f(uint16_t{});
+  else f(_Float16{});
+}
+}  // namespace lin
+}  // namespace rtseg
