@@ -35,13 +35,16 @@ __device__ __forceinline__ float normal_tail(float a) {
   return __builtin_amdgcn_exp2f(__builtin_fmaf(a, q, -0.9999992251396179f));
 }
 // gelu(x) = x Phi(x) = max(x, 0) - |x| Phi(-|x|), gelu'(x) = Phi(x) + x phi(x).  16-bit operands take the tail
-// above (10 full-rate instructions and one quarter-rate; erff costs five times that, and the activation is
-// what bounds the wide layers' forward); fp32 ones erff.
+// above (11 full-rate instructions and one quarter-rate; erff costs five times that, and the activation is
+// what bounds the wide layers' forward); fp32 ones erff.  max and min work on the bits: the float forms
+// spend an instruction each to quiet a NaN, which here comes through the tail.
 template <typename T>
 __device__ __forceinline__ float gelu(float x) {
   if constexpr (sizeof(T) == 4) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-  const float ax = fabsf(x);  // the factor is cut off where the tail is 0: inf - inf * 0 is inf
-  return __builtin_fmaf(-fminf(ax, 64.f), normal_tail(ax), fmaxf(x, 0.f));
+  const int bits = __float_as_int(x);
+  // the factor is cut off at 64, where the tail is 0: inf - inf * 0 is inf
+  const float a = __int_as_float(min(bits & 0x7fffffff, 0x42800000));
+  return __builtin_fmaf(-a, normal_tail(fabsf(x)), __int_as_float(max(bits, 0)));
 }
 template <typename T>
 __device__ __forceinline__ float gelu_slope(float x) {
@@ -189,5 +192,19 @@ void by_type(int dt, F f) {
   else if (dt == kBF16) f(uint16_t{});
   else f(_Float16{});
 }
+// Blocks that the whole device holds at once, for kernels whose blocks walk over several tiles.
+template <class K>
+int resident_blocks(K kernel, int threads) {
+  int a_cu = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&a_cu, kernel, threads, 0) != hipSuccess || a_cu < 1) a_cu = 2;
+  return 256 * a_cu;
+}
+// A grid of at most that many blocks, a multiple of ntiles, each with the same number of row tiles: one
+// block more than fit would cost as long again as all the others.
+inline unsigned one_wave_grid(int resident, int mtiles, int ntiles) {
+  const int most = resident / ntiles > 0 ? resident / ntiles : 1, each = (mtiles + most - 1) / most;
+  return static_cast<unsigned>((mtiles + each - 1) / each * ntiles);
+}
+
 }  // namespace lin
 }  // namespace rtseg

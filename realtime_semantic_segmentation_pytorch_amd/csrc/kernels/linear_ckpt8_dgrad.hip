@@ -304,10 +304,9 @@ void launch_cfg(DgradArgs p, hipStream_t st) {
   if constexpr (WK == 1 && VEC) {
     if (p.R <= 8 * kPer16<T>) {
       constexpr int W1 = ACT == kCkptGelu && TM == 4 && WAVES > 2 ? WAVES - 1 : WAVES;  // more registers
-      // about four blocks a CU, each with the same number of tiles
-      const int most = 1024 / p.ntiles > 0 ? 1024 / p.ntiles : 1, each = (p.mtiles + most - 1) / most;
-      const unsigned grid = static_cast<unsigned>((p.mtiles + each - 1) / each * p.ntiles);
-      lin_dgrad_kernel<T, ACT, WN, WM, WK, TM, true, VEC, W1><<<grid, WN * WM * WK * 64, 0, st>>>(p);
+      const auto kernel = lin_dgrad_kernel<T, ACT, WN, WM, WK, TM, true, VEC, W1>;
+      static const int resident = resident_blocks(kernel, WN * WM * WK * 64);
+      kernel<<<one_wave_grid(resident, p.mtiles, p.ntiles), WN * WM * WK * 64, 0, st>>>(p);
       return;
     }
   }

@@ -79,8 +79,18 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_fwd_kernel(const F
       }
     }
   };
+  // its codes: the lane's part of the address, and the scale byte's (one lane a block)
+  uint32_t coff[XA], eoff[XA];
+#pragma unroll
+  for (int i = 0; i < XA; ++i) {
+    const uint32_t row = lrow + (WK == 1 ? NT / 8 * i : 0);
+    coff[i] = row * p.Cp + lk;
+    eoff[i] = lk % kBlock == 0 ? row * (p.Cp / kBlock) + lk / kBlock : kOut;
+  }
   auto stage_a = [&](int m, int k0, int buf) {
     const int64_t m0 = static_cast<int64_t>(m) * BM;
+    const __amdgpu_buffer_rsrc_t cr = range(p.codes + m0 * p.Cp, (p.M - m0) * p.Cp);
+    const __amdgpu_buffer_rsrc_t er = range(p.scales + m0 * (p.Cp / kBlock), (p.M - m0) * (p.Cp / kBlock));
 #pragma unroll
     for (int i = 0; i < XA; ++i) {
       const int slot = srow + NT / 8 * i, row = slot % BM;
@@ -95,15 +105,19 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_fwd_kernel(const F
           const uint32_t top = top_bits<T>(ra[i], v);
           const uint32_t byte = scale_byte(PER == 8 ? quad_max(top) : oct_max(top));
           const float inv = inv_scale(byte);
-          if (m0 + row < p.M && k < p.Cp) {
-            const int64_t o = (m0 + row) * p.Cp + k;
-            uint32_t c[PER / 4];
-            // a NaN that was widened from 16 bits has a low byte of 0, and so has inf * 0: no code to clear
+          // a NaN that was widened from 16 bits has a low byte of 0, and so has inf * 0: no code to clear
+          uint32_t c[PER / 4];
 #pragma unroll
-            for (int e = 0; e < PER / 4; ++e) c[e] = code4(v + 4 * e, inv, ES == 4 && byte == 255u);
-            __builtin_memcpy(__builtin_assume_aligned(p.codes + o, PER), c, PER);
-            if (k % kBlock == 0) p.scales[o / kBlock] = static_cast<uint8_t>(byte);
+          for (int e = 0; e < PER / 4; ++e) c[e] = code4(v + 4 * e, inv, ES == 4 && byte == 255u);
+          const int kc = k0 + (WK == 1 ? 0 : NT / 8 * i / BM * BK);
+          const bool in = kc + lk < p.Cp;
+          if constexpr (PER == 8) {
+            const u32x2_t two = {c[0], c[1]};
+            __builtin_amdgcn_raw_buffer_store_b64(two, cr, static_cast<int>(in ? coff[i] : kOut), kc, 0);
+          } else {
+            __builtin_amdgcn_raw_buffer_store_b32(c[0], cr, static_cast<int>(in ? coff[i] : kOut), kc, 0);
           }
+          __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(byte), er, static_cast<int>(in ? eoff[i] : kOut), kc / kBlock, 0);
         }
         if constexpr (ACT == kCkptGelu) {
 #pragma unroll
@@ -268,10 +282,9 @@ void launch_cfg(FwdArgs p, hipStream_t st) {
   if constexpr (WK == 1 && VEC && BN <= 256) {
     if (p.K <= 8 * kPer16<T>) {
       constexpr int W1 = ACT == kCkptGelu && WAVES > 2 ? WAVES - 1 : WAVES;  // more registers
-      // about four blocks a CU, each with the same number of tiles
-      const int most = 1024 / p.ntiles > 0 ? 1024 / p.ntiles : 1, each = (p.mtiles + most - 1) / most;
-      const unsigned grid = static_cast<unsigned>((p.mtiles + each - 1) / each * p.ntiles);
-      lin_fwd_kernel<T, ACT, WN, WM, WK, TM, TN, true, VEC, W1><<<grid, WN * WM * WK * 64, 0, st>>>(p);
+      const auto kernel = lin_fwd_kernel<T, ACT, WN, WM, WK, TM, TN, true, VEC, W1>;
+      static const int resident = resident_blocks(kernel, WN * WM * WK * 64);
+      kernel<<<one_wave_grid(resident, p.mtiles, p.ntiles), WN * WM * WK * 64, 0, st>>>(p);
       return;
     }
   }
