@@ -70,67 +70,5 @@ __device__ __forceinline__ uint2 encode8(const float* v, uint32_t& byte) {
   return make_uint2(code4(v, inv, byte == 255u), code4(v + 4, inv, byte == 255u));
 }
 
-// ---- eight consecutive channels of a row, as raw bits and as floats ----------------------------
-template <typename T> struct Raw8 { uint4 q[sizeof(T) / 2]; };
-
-// n: channels from p on that exist (<= 0: none); vec: p is 16-byte aligned and n is 0 or >= 8
-template <typename T>
-__device__ __forceinline__ Raw8<T> load8(const T* p, int n, bool vec) {
-  Raw8<T> r;
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.q[i] = make_uint4(0u, 0u, 0u, 0u);
-  if (vec) {
-    if (n > 0) {
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.q[i] = reinterpret_cast<const uint4*>(p)[i];
-    }
-  } else {
-    T t[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      t[i] = T(0);
-      if (i < n) t[i] = p[i];
-    }
-    __builtin_memcpy(&r, t, sizeof(t));
-  }
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void unraw8(const Raw8<T>& r, float* v) {
-  T t[8];
-  __builtin_memcpy(t, &r, sizeof(t));
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = Io<T>::ld(t + i);
-}
-template <typename T>
-__device__ __forceinline__ Raw8<T> raw8(const float* v) {
-  Raw8<T> r;
-  if constexpr (sizeof(T) == 2 && !__is_same(T, _Float16)) {
-    r.q[0] = make_uint4(f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]),
-                        f32x2_to_bf16x2(v[6], v[7]));
-  } else {
-    T t[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) Io<T>::st(t + i, v[i]);
-    __builtin_memcpy(&r, t, sizeof(t));
-  }
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const Raw8<T>& r, int n, bool vec) {
-  if (vec) {
-    if (n > 0) {
-#pragma unroll
-      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.q[i];
-    }
-  } else {
-    T t[8];
-    __builtin_memcpy(t, &r, sizeof(t));
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) p[i] = t[i];
-  }
-}
-
 }  // namespace ckpt8
 }  // namespace rtseg

@@ -441,7 +441,7 @@ void launch_ckpt8_pack(const void* x, int dtype, int8_t* codes, uint8_t* scales,
 void launch_ckpt8_unpack(const int8_t* codes, const uint8_t* scales, void* x, int dtype, int64_t rows, int C,
                          hipStream_t st);
 
-// ---- layer_norm.hip ---------------------------------------------------------------
+// ---- layer_norm_*.hip ---------------------------------------------------------------
 // All tensors are contiguous [rows, C]; 1 <= C <= layer_norm_max_channels().  The output type is the
 // stream's, fp32, or 16 bits behind an fp32 stream; the branch r is of the stream's type, or 16 bits
 // behind an fp32 stream.
@@ -462,7 +462,6 @@ struct LnFwdArgs {
   int64_t Cp;
   float eps;
   int lanes;          // set by the launcher
-  bool vec, wvec;
 };
 struct LnBwdArgs {
   const void* dy;
@@ -481,14 +480,13 @@ struct LnBwdArgs {
   int C;
   int64_t Cp;
   int lanes, blocks;  // set by the launcher
-  bool vec, wvec;
 };
 int layer_norm_max_channels();
 int layer_norm_bwd_blocks(int64_t rows, int C);
 void launch_layer_norm_fwd(LnFwdArgs a, hipStream_t st);
 void launch_layer_norm_bwd(LnBwdArgs a, float* dw, float* db, hipStream_t st);
 
-// ---- linear_ckpt8.hip ---------------------------------------------------------------
+// ---- linear_ckpt8_*.hip ---------------------------------------------------------------
 // y = act(x) w^T + b for x [M, K], w [N, K]; the checkpoint of x is written by the forward and read by
 // both gradients.  x / y / dy / dx / w are of one type (fp32 / bf16 / fp16); b that type or fp32.
 enum CkptAct : int { kCkptNone = 0, kCkptGelu = 1 };

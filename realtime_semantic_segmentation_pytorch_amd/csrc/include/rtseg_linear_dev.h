@@ -13,11 +13,13 @@
 #include "rtseg_ckpt8.h"
 #include "rtseg_launch.h"
 #include "rtseg_mfma_dev.h"
+#include "rtseg_rows_dev.h"
 
 namespace rtseg {
 namespace lin {
 
 using namespace ckpt8;
+using namespace rows;
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
@@ -54,9 +56,6 @@ __device__ __forceinline__ float gelu_slope(float x) {
   return __builtin_fmaf(x * 0.39894228040143268f, e, x >= 0.f ? 1.f - tail : tail);
 }
 
-// 16 bytes of operand: 8 (bf16 / fp16) or 4 (fp32) consecutive k
-template <typename T> constexpr int kPer16 = 16 / static_cast<int>(sizeof(T));
-
 template <typename T>
 __device__ __forceinline__ void unpack16(uint4 q, float* v) {
   T t[kPer16<T>];
@@ -79,30 +78,6 @@ __device__ __forceinline__ uint4 pack16<uint16_t>(const float* v) {
                     f32x2_to_bf16x2(v[6], v[7]));
 }
 
-// A range of a tensor as a buffer: loads past `bytes` read 0 and stores there are dropped, so the rows
-// that a tile does not have cost no branch.  kOut as an offset is past every range.
-constexpr uint32_t kOut = 0xfffffff0u;
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t range(const void* p, int64_t bytes) {
-  const uint32_t n = bytes < 0 ? 0u : bytes > 0xffffff00ll ? 0xffffff00u : static_cast<uint32_t>(bytes);
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(n), 0x00020000);
-}
-typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
-// `off` alone decides whether an access is in range; `base` (uniform, added to it) only moves along a row,
-// between columns that the caller has checked, so that a range has to end at the last row and no sooner
-__device__ __forceinline__ uint4 buf16(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t base = 0) {
-  return __builtin_bit_cast(
-      uint4, static_cast<u32x4_t>(__builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(off), static_cast<int>(base), 0)));
-}
-__device__ __forceinline__ uint8_t buf1(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t base = 0) {
-  return static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(r, static_cast<int>(off), static_cast<int>(base), 0));
-}
-__device__ __forceinline__ void put16(__amdgpu_buffer_rsrc_t r, uint32_t off, uint4 v) {
-  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), r, static_cast<int>(off), 0, 0);
-}
-__device__ __forceinline__ void put8(__amdgpu_buffer_rsrc_t r, uint32_t off, uint2 v) {
-  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, v), r, static_cast<int>(off), 0, 0);
-}
 // four values of a 16-bit T
 template <typename T>
 __device__ __forceinline__ uint2 pack8(const float* v) {
@@ -113,32 +88,6 @@ __device__ __forceinline__ uint2 pack8(const float* v) {
   } else {
     return make_uint2(f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]));
   }
-}
-
-// Rows of any alignment.  The load is issued without a branch, from inside the tensor: p[i] where 16 bytes
-// fit behind it, else from its last 16 bytes (the tensor has at least that many where a row does; rows that
-// are shorter are left to settle16).  A value for which fewer than 16 bytes exist is settled when it is
-// used, after the wait: 0 where nothing exists, a row's last elements one by one.
-template <typename T>
-__device__ __forceinline__ uint4 any16(const T* p, int64_t i, int64_t size) {
-  uint4 q = make_uint4(0u, 0u, 0u, 0u);
-  const int64_t last = size - kPer16<T>;
-  if (last >= 0) __builtin_memcpy(&q, p + (i < last ? i : last), 16);
-  return q;
-}
-template <typename T>
-__device__ __forceinline__ uint4 settle16(uint4 q, const T* p, int64_t i, int n) {
-  if (n <= 0) return make_uint4(0u, 0u, 0u, 0u);
-  if (n < kPer16<T>) {
-    T t[kPer16<T>];
-#pragma unroll
-    for (int e = 0; e < kPer16<T>; ++e) {
-      t[e] = T(0);
-      if (e < n) t[e] = p[i + e];
-    }
-    __builtin_memcpy(&q, t, 16);
-  }
-  return q;
 }
 
 // largest of the chunk's absolute values as the bits of an fp32, NaN above infinity above every number
@@ -184,7 +133,6 @@ __device__ __forceinline__ uint2 tr_read(const void* p) {
 // the 16 rows of a fragment read over the banks
 __device__ __forceinline__ int swz_a(int row) { return row & 7; }
 
-inline bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 inline int elem(int dt) { return dt == kF32 ? 4 : 2; }
 template <class F>
 void by_type(int dt, F f) {

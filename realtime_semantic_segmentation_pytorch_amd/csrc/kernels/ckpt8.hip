@@ -3,35 +3,53 @@
 // Both are one pass over the data and bound by HBM: 8 channels a lane (16 or 32 bytes), the block
 // maximum of 32 channels across 4 lanes by two DPP moves, no LDS.  A lane keeps two rows' worth of
 // loads in flight through the grid's many waves; nothing is reused, so there is nothing to tile.
+#include <type_traits>
+
 #include "rtseg_ckpt8.h"
 #include "rtseg_launch.h"
+#include "rtseg_rows_dev.h"
 
 namespace rtseg {
 namespace {
 
 using namespace ckpt8;
+using namespace rows;
 
 // item = 8 channels of the padded row: items_row = Cp / 8 per row, 4 consecutive items = one block
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) ckpt8_pack_kernel(const T* __restrict__ x, uint2* __restrict__ codes,
-                                                         uint8_t* __restrict__ scales, int64_t items, int C,
-                                                         int items_row, bool vec) {
+                                                         uint8_t* __restrict__ scales, int64_t items, int64_t rows, int C,
+                                                         int items_row) {
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
   for (int64_t it = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; it < items; it += step) {
     const int64_t row = it / items_row;
     const int c = static_cast<int>(it - row * items_row) * 8;
+    const int n = C - c;
+    Raw8<T> r;
     float v[8];
-    unraw8<T>(load8<T>(x + row * C + c, C - c, vec), v);
+    if constexpr (VEC) {  // a lane behind the last channel reads its row's first ones and drops them
+      const uint4* p = reinterpret_cast<const uint4*>(x + row * C + (n > 0 ? c : 0));
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
+        r.q[i] = p[i];
+        if (n <= 0) r.q[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    } else {
+      const Span<T, false> s(x, row * C, rows * C);
+      r = s.load(c, n);
+      s.settle(r, c, n);
+    }
+    unraw8<T>(r, v);
     uint32_t byte;
     codes[it] = encode8(v, byte);  // items is a multiple of 4: a block's lanes leave the loop together
     if ((it & 3) == 0) scales[it >> 2] = static_cast<uint8_t>(byte);
   }
 }
 
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) ckpt8_unpack_kernel(const uint2* __restrict__ codes,
                                                            const uint8_t* __restrict__ scales, T* __restrict__ x,
-                                                           int64_t items, int C, int items_row, bool vec) {
+                                                           int64_t items, int64_t rows, int C, int items_row) {
   const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
   for (int64_t it = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; it < items; it += step) {
     const int64_t row = it / items_row;
@@ -41,11 +59,30 @@ __global__ void __launch_bounds__(256) ckpt8_unpack_kernel(const uint2* __restri
     float v[8];
     decode4(w.x, s, v);
     decode4(w.y, s, v + 4);
-    store8<T>(x + row * C + c, raw8<T>(v), C - c, vec);
+    const Raw8<T> r = raw8<T>(v);
+    if constexpr (VEC) {
+      if (c < C) {
+        uint4* p = reinterpret_cast<uint4*>(x + row * C + c);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) p[i] = r.q[i];
+      }
+    } else {
+      Span<T, false>(x, row * C, rows * C).store(c, C - c, r);
+    }
   }
 }
 
-bool vec_ok(const void* p, int C) { return C % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// f(T{}, are the rows 16-byte aligned?)
+template <class F>
+void by_rows(int dtype, const void* p, int C, F f) {
+  auto with = [&](auto t) {
+    if (C % 8 == 0 && al16(p)) f(t, std::true_type{});
+    else f(t, std::false_type{});
+  };
+  if (dtype == kF32) with(float{});
+  else if (dtype == kBF16) with(uint16_t{});
+  else with(_Float16{});
+}
 
 }  // namespace
 
@@ -54,13 +91,11 @@ void launch_ckpt8_pack(const void* x, int dtype, int8_t* codes, uint8_t* scales,
   const int64_t items = rows * per;
   if (items == 0) return;
   const int grid = stream_grid(items, 256);
-  const bool vec = vec_ok(x, C);
-  auto* cd = reinterpret_cast<uint2*>(codes);
-  switch (dtype) {
-    case kF32: ckpt8_pack_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(x), cd, scales, items, C, per, vec); break;
-    case kBF16: ckpt8_pack_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(x), cd, scales, items, C, per, vec); break;
-    default: ckpt8_pack_kernel<<<grid, 256, 0, st>>>(static_cast<const _Float16*>(x), cd, scales, items, C, per, vec); break;
-  }
+  by_rows(dtype, x, C, [&](auto t, auto vec) {
+    using T = decltype(t);
+    constexpr auto kernel = &ckpt8_pack_kernel<T, decltype(vec)::value>;
+    kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(x), reinterpret_cast<uint2*>(codes), scales, items, rows, C, per);
+  });
 }
 
 void launch_ckpt8_unpack(const int8_t* codes, const uint8_t* scales, void* x, int dtype, int64_t rows, int C,
@@ -69,13 +104,11 @@ void launch_ckpt8_unpack(const int8_t* codes, const uint8_t* scales, void* x, in
   const int64_t items = rows * per;
   if (items == 0) return;
   const int grid = stream_grid(items, 256);
-  const bool vec = vec_ok(x, C);
-  const auto* cd = reinterpret_cast<const uint2*>(codes);
-  switch (dtype) {
-    case kF32: ckpt8_unpack_kernel<<<grid, 256, 0, st>>>(cd, scales, static_cast<float*>(x), items, C, per, vec); break;
-    case kBF16: ckpt8_unpack_kernel<<<grid, 256, 0, st>>>(cd, scales, static_cast<uint16_t*>(x), items, C, per, vec); break;
-    default: ckpt8_unpack_kernel<<<grid, 256, 0, st>>>(cd, scales, static_cast<_Float16*>(x), items, C, per, vec); break;
-  }
+  by_rows(dtype, x, C, [&](auto t, auto vec) {
+    using T = decltype(t);
+    constexpr auto kernel = &ckpt8_unpack_kernel<T, decltype(vec)::value>;
+    kernel<<<grid, 256, 0, st>>>(reinterpret_cast<const uint2*>(codes), scales, static_cast<T*>(x), items, rows, C, per);
+  });
 }
 
 }  // namespace rtseg
