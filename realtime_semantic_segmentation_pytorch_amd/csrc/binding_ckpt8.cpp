@@ -1,5 +1,5 @@
 // torch.library registration of the layer norm, the 8-bit activation checkpoints and the linear layer
-// that keeps one (layer_norm.hip, ckpt8.hip, linear_ckpt8.hip).  The two differentiable ones have their
+// that keeps one (layer_norm_*.hip, ckpt8.hip, linear_ckpt8_*.hip).  The two differentiable ones have their
 // autograd node here, not in Python: a training step of a small layer is bound by the host, and the
 // Python nodes cost 30 us of the 125 us that forward and backward of 32 x 256 x 256 took.
 #include <ATen/ATen.h>
@@ -90,10 +90,11 @@ void check_ln_types(int x, int y, const char* op) {
   TORCH_CHECK(y == x || y == 0 || x == 0, "rtseg.", op, ": the output is of the input's type, fp32, or 16 bits behind fp32");
 }
 
-// keep: 0 nothing, 1 mean / rstd, 2 those and the 8-bit checkpoint.  -> (sum or empty, y, mean, rstd, codes, scales)
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
+// keep: 0 nothing, 1 mean / rstd ([2, rows]), 2 those and the 8-bit checkpoint.  -> (sum or empty, y, stats, codes,
+// scales), the first two of `shape` (x's rows as the caller has them: a result that is a view could not be changed in place)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> layer_norm_fwd(
     const at::Tensor& x, const std::optional<at::Tensor>& r, const std::optional<at::Tensor>& w,
-    const std::optional<at::Tensor>& b, double eps, at::ScalarType out, int64_t keep, bool want_sum) {
+    const std::optional<at::Tensor>& b, double eps, at::ScalarType out, int64_t keep, bool want_sum, at::IntArrayRef shape) {
   check_rows(x, "layer_norm", "x");
   const int64_t rows = x.size(0), C = x.size(1);
   TORCH_CHECK(C <= layer_norm_max_channels(), "rtseg.layer_norm: at most ", layer_norm_max_channels(), " channels");
@@ -101,7 +102,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   LnFwdArgs a{};
   a.x = x.data_ptr();
   a.x_dtype = dtype_code(x);
-  at::Tensor s, y = at::empty({rows, C}, x.options().dtype(out));
+  at::Tensor s, y = at::empty(shape, x.options().dtype(out));
   a.y = y.data_ptr();
   a.y_dtype = dtype_code(y);
   check_ln_types(a.x_dtype, a.y_dtype, "layer_norm");
@@ -113,7 +114,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     TORCH_CHECK(a.r_dtype == a.x_dtype || a.x_dtype == 0,
                 "rtseg.layer_norm: residual must be of x's type, or 16 bits beside an fp32 x");
     if (want_sum) {
-      s = at::empty_like(x);
+      s = at::empty(shape, x.options());
       a.s = s.data_ptr();
     }
   }
@@ -124,12 +125,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
                   "rtseg.layer_norm: weight and bias must be contiguous fp32 [", C, "] on x's device");
   a.w = static_cast<const float*>(opt_ptr(w));
   a.b = static_cast<const float*>(opt_ptr(b));
-  at::Tensor mean, rstd, codes, scales;
+  at::Tensor stats, codes, scales;
   if (keep > 0) {
-    mean = at::empty({rows}, x.options().dtype(at::kFloat));
-    rstd = at::empty_like(mean);
-    a.mean = mean.data_ptr<float>();
-    a.rstd = rstd.data_ptr<float>();
+    stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
+    a.mean = stats.data_ptr<float>();
+    a.rstd = a.mean + rows;
   }
   if (keep > 1) {
     std::tie(codes, scales) = new_ckpt(rows, C, x);
@@ -141,15 +141,15 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
   a.Cp = padded(C);
   a.eps = static_cast<float>(eps);
   launch_layer_norm_fwd(a, cur_stream());
-  return {s, y, mean, rstd, codes, scales};
+  return {s, y, stats, codes, scales};
 }
 
 // -> (dx or empty, dr, dw, db or empty).  dr is written only where the branch's type is not the
 // stream's: where it is, its gradient is dx.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd(
     const at::Tensor& dy, const std::optional<at::Tensor>& ds, const std::optional<at::Tensor>& x,
-    const std::optional<at::Tensor>& codes, const std::optional<at::Tensor>& scales, const at::Tensor& mean,
-    const at::Tensor& rstd, const std::optional<at::Tensor>& w, at::ScalarType x_dtype,
+    const std::optional<at::Tensor>& codes, const std::optional<at::Tensor>& scales, const at::Tensor& stats,
+    const std::optional<at::Tensor>& w, at::ScalarType x_dtype,
     std::optional<at::ScalarType> r_dtype, bool want_dx, bool want_dr, bool want_w) {
   check_rows(dy, "layer_norm_bwd", "grad");
   const int64_t rows = dy.size(0), C = dy.size(1);
@@ -180,12 +180,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> layer_norm_bwd(
                 "rtseg.layer_norm_bwd: the gradient of the sum must be of the sum's shape and type");
     a.ds = ds->data_ptr();
   }
-  for (const auto* p : {&mean, &rstd})
-    TORCH_CHECK(p->is_cuda() && p->device() == dy.device() && p->scalar_type() == at::kFloat && p->is_contiguous() &&
-                    p->dim() == 1 && p->size(0) == rows,
-                "rtseg.layer_norm_bwd: mean and rstd must be contiguous fp32 [rows]");
-  a.mean = mean.data_ptr<float>();
-  a.rstd = rstd.data_ptr<float>();
+  TORCH_CHECK(stats.is_cuda() && stats.device() == dy.device() && stats.scalar_type() == at::kFloat &&
+                  stats.is_contiguous() && stats.numel() == 2 * rows,
+              "rtseg.layer_norm_bwd: mean and rstd must be contiguous fp32 [2, rows]");
+  a.mean = stats.data_ptr<float>();
+  a.rstd = a.mean + rows;
   if (w.has_value()) {
     TORCH_CHECK(w->is_cuda() && w->device() == dy.device() && w->scalar_type() == at::kFloat && w->is_contiguous() &&
                     w->dim() == 1 && w->size(0) == C,
@@ -222,7 +221,8 @@ int act_code(int64_t act) {
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ckpt8_fwd(const at::Tensor& x, const at::Tensor& w,
-                                                                const std::optional<at::Tensor>& b, int64_t act, bool keep) {
+                                                                const std::optional<at::Tensor>& b, int64_t act, bool keep,
+                                                                at::IntArrayRef shape) {
   check_rows(x, "linear_ckpt8", "x");
   TORCH_CHECK(w.dim() == 2 && w.size(0) >= 1 && w.size(0) <= kMaxChannels && w.scalar_type() == x.scalar_type(),
               "rtseg.linear_ckpt8: weight must be [out, in] of x's type with 1 .. ", kMaxChannels, " outputs");
@@ -230,7 +230,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ckpt8_fwd(const at::Tensor
   check_param(w, {N, K}, x, "linear_ckpt8", "weight");
   if (b.has_value()) check_param(*b, {N}, x, "linear_ckpt8", "bias");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
-  at::Tensor y = at::empty({M, N}, x.options()), codes, scales;
+  at::Tensor y = at::empty(shape, x.options()), codes, scales;
   LinFwdArgs a{};
   if (keep) {
     std::tie(codes, scales) = new_ckpt(M, K, x);
@@ -326,7 +326,10 @@ at::Tensor linear_ckpt8_bgrad(const at::Tensor& dy, at::ScalarType dtype) {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-at::Tensor rows_of(const at::Tensor& t) { return t.reshape({-1, t.size(-1)}).contiguous(); }
+at::Tensor rows_of(const at::Tensor& t) {
+  return t.dim() == 2 && t.is_contiguous() ? t : t.reshape({-1, t.size(-1)}).contiguous();
+}
+at::Tensor shaped(const at::Tensor& t, at::IntArrayRef sizes) { return t.sizes() == sizes ? t : t.view(sizes); }
 
 // The gradients are kernels' outputs without a graph of their own: under create_graph any further use
 // of them raises instead of passing for a constant.
@@ -349,29 +352,30 @@ struct LinearCkpt8Fn : torch::autograd::Function<LinearCkpt8Fn> {
                             const std::optional<at::Tensor>& b, int64_t act, bool need_x, bool need_w, bool need_b) {
     // fp32 weights beside 16-bit operands are cast once, for the forward and the data gradient
     const at::Tensor x2 = rows_of(x), wc = w.to(x.scalar_type()).contiguous();
-    auto [y, codes, scales] = linear_ckpt8_fwd(x2, wc, b, act, need_w || (need_x && act != kCkptNone));
+    auto shape = x.sizes().vec();
+    if (need_x) ctx->saved_data["shape"] = shape;
+    shape.back() = w.size(0);
+    auto [y, codes, scales] = linear_ckpt8_fwd(x2, wc, b, act, need_w || (need_x && act != kCkptNone), shape);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({codes, scales, need_x ? wc : at::Tensor()});
-    ctx->saved_data["k"] = x2.size(1);
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["need"] = static_cast<int64_t>(need_x | need_w << 1 | need_b << 2);
-    ctx->saved_data["wt"] = static_cast<int64_t>(w.scalar_type());
-    auto shape = x.sizes().vec();
-    ctx->saved_data["shape"] = shape;
-    shape.back() = w.size(0);
-    return y.view(shape);
+    ctx->saved_data["call"] = std::vector<int64_t>{x2.size(1), act, need_x, need_w, need_b, static_cast<int64_t>(w.scalar_type())};
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(7);
     if (!grads[0].defined()) return out;
     const variable_list saved = ctx->get_saved_variables();
-    const int64_t need = ctx->saved_data["need"].toInt(), act = ctx->saved_data["act"].toInt(), k = ctx->saved_data["k"].toInt();
-    const auto wt = static_cast<at::ScalarType>(ctx->saved_data["wt"].toInt());
-    const at::Tensor dy = rows_of(grads[0].detach());
-    if (need & 1)
-      out[0] = linear_ckpt8_dgrad(dy, saved[2], maybe(saved[0]), maybe(saved[1]), act).view(ctx->saved_data["shape"].toIntVector());
-    if (need & 2) std::tie(out[1], out[2]) = linear_ckpt8_wgrad(dy, saved[0], saved[1], k, act, wt, need & 4);
-    else if (need & 4) out[2] = linear_ckpt8_bgrad(dy, wt);
+    const auto call = ctx->saved_data["call"].toIntVector();
+    const int64_t k = call[0], act = call[1];
+    const bool need_x = call[2] != 0, need_w = call[3] != 0, need_b = call[4] != 0;
+    const auto wt = static_cast<at::ScalarType>(call[5]);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor dy = rows_of(grads[0]);
+    if (need_x)
+      out[0] = shaped(linear_ckpt8_dgrad(dy, saved[2], maybe(saved[0]), maybe(saved[1]), act),
+                      ctx->saved_data["shape"].toIntVector());
+    if (need_w) std::tie(out[1], out[2]) = linear_ckpt8_wgrad(dy, saved[0], saved[1], k, act, wt, need_b);
+    else if (need_b) out[2] = linear_ckpt8_bgrad(dy, wt);
     return once(std::move(out));
   }
 };
@@ -380,7 +384,7 @@ at::Tensor linear_ckpt8(const at::Tensor& x, const at::Tensor& w, const std::opt
   const at::Tensor x2 = rows_of(x);
   auto shape = x.sizes().vec();
   shape.back() = w.size(0);
-  return std::get<0>(linear_ckpt8_fwd(x2, w.to(x.scalar_type()).contiguous(), b, act, false)).view(shape);
+  return std::get<0>(linear_ckpt8_fwd(x2, w.to(x.scalar_type()).contiguous(), b, act, false, shape));
 }
 at::Tensor linear_ckpt8_autograd(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& b, int64_t act) {
   const bool on = at::GradMode::is_enabled();
@@ -403,30 +407,31 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     if (w.has_value()) wf = w->to(at::kFloat).contiguous();
     if (b.has_value()) bf = b->to(at::kFloat).contiguous();
     // without a checkpoint the backward normalises the sum again, so it is kept even if unwanted
-    auto [s, y, mean, rstd, codes, scales] = layer_norm_fwd(x2, r2, wf, bf, eps, out, need == 0 ? 0 : ckpt ? 2 : 1, sum || !ckpt);
-    ctx->set_materialize_grads(false);
-    ctx->save_for_backward({ckpt ? codes : r.has_value() ? s : x2, scales, mean, rstd, wf.has_value() ? *wf : at::Tensor()});
-    ctx->saved_data["need"] = need;
-    ctx->saved_data["ckpt"] = ckpt;
-    ctx->saved_data["sum"] = sum;
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["xt"] = static_cast<int64_t>(x.scalar_type());
-    ctx->saved_data["rt"] = static_cast<int64_t>(r.has_value() ? r->scalar_type() : x.scalar_type());
-    ctx->saved_data["wt"] = static_cast<int64_t>(w.has_value() ? w->scalar_type() : at::kFloat);
-    ctx->saved_data["bt"] = static_cast<int64_t>(b.has_value() ? b->scalar_type() : at::kFloat);
+    auto [s, y, stats, codes, scales] = layer_norm_fwd(x2, r2, wf, bf, eps, out, need == 0 ? 0 : ckpt ? 2 : 1, sum || !ckpt,
+                                                      x.sizes());
+    auto st = [](const std::optional<at::Tensor>& t, at::ScalarType other) {
+      return static_cast<int64_t>(t.has_value() ? t->scalar_type() : other);
+    };
     variable_list got;
-    if (sum) got.push_back(s.view(x.sizes()));
-    got.push_back(y.view(x.sizes()));
+    if (sum) got.push_back(s);
+    got.push_back(y);
+    // the tensor that the caller holds, where there is one, not a view of it: a change in place has to be noticed
+    const at::Tensor kept = ckpt ? codes : r.has_value() ? s : x.is_contiguous() ? x : x2;
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({kept, scales, stats, wf.has_value() ? *wf : at::Tensor()});
+    ctx->saved_data["call"] = std::vector<int64_t>{need, ckpt, sum, static_cast<int64_t>(x.scalar_type()), st(r, x.scalar_type()),
+                                                   st(w, at::kFloat), st(b, at::kFloat)};
+    ctx->saved_data["shape"] = x.sizes().vec();
     return got;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     variable_list out(9);
-    auto& d = ctx->saved_data;
-    const int64_t need = d["need"].toInt();
-    const bool need_x = need & 1, need_r = need & 2, need_w = need & 4, need_b = need & 8, ckpt = d["ckpt"].toBool();
-    auto type = [&](const char* k) { return static_cast<at::ScalarType>(d[k].toInt()); };
-    const at::ScalarType xt = type("xt"), rt = type("rt");
-    const at::Tensor ds = d["sum"].toBool() ? grads[0] : at::Tensor(), dy = grads.back();
+    const auto call = ctx->saved_data["call"].toIntVector();
+    const int64_t need = call[0];
+    const bool need_x = need & 1, need_r = need & 2, need_w = need & 4, need_b = need & 8, ckpt = call[1] != 0, sum = call[2] != 0;
+    auto type = [&](int i) { return static_cast<at::ScalarType>(call[i]); };
+    const at::ScalarType xt = type(3), rt = type(4);
+    const at::Tensor ds = sum ? grads[0] : at::Tensor(), dy = grads.back();
     if (!dy.defined()) {  // the norm's output is unused: only the sum carries a gradient
       if (ds.defined() && need_x) out[0] = ds;
       if (ds.defined() && need_r) out[1] = ds.to(rt);
@@ -434,17 +439,22 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     }
     const variable_list saved = ctx->get_saved_variables();
     const bool own_r = need_r && rt != xt;
-    std::optional<at::Tensor> ds2;
-    if (ds.defined()) ds2 = rows_of(ds.detach());
-    auto [dx, dr, dw, db] = layer_norm_bwd(rows_of(dy.detach()), ds2, ckpt ? std::nullopt : maybe(saved[0]),
-                                           ckpt ? maybe(saved[0]) : std::nullopt, ckpt ? maybe(saved[1]) : std::nullopt,
-                                           saved[2], saved[3], maybe(saved[4]), xt, rt, need_x || (need_r && !own_r), own_r,
-                                           need_w || need_b);
-    const auto shape = d["shape"].toIntVector();
-    if (need_x) out[0] = dx.view(shape);
-    if (need_r) out[1] = (own_r ? dr : dx).view(shape);
-    if (need_w) out[2] = dw.to(type("wt"));
-    if (need_b) out[3] = db.to(type("bt"));
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::optional<at::Tensor> ds2, x2;
+      if (ds.defined()) ds2 = rows_of(ds);
+      if (!ckpt) x2 = rows_of(saved[0]);
+      auto [dx, dr, dw, db] = layer_norm_bwd(rows_of(dy), ds2, x2, ckpt ? maybe(saved[0]) : std::nullopt,
+                                             ckpt ? maybe(saved[1]) : std::nullopt, saved[2], maybe(saved[3]), xt, rt,
+                                             need_x || (need_r && !own_r), own_r, need_w || need_b);
+      const auto shape = ctx->saved_data["shape"].toIntVector();
+      if (dx.defined()) dx = shaped(dx, shape);
+      // one tensor, not two views of it: whoever accumulates into the one then knows that it is shared
+      if (need_x) out[0] = dx;
+      if (need_r) out[1] = own_r ? shaped(dr, shape) : dx;
+      if (need_w) out[2] = dw.to(type(5));
+      if (need_b) out[3] = db.to(type(6));
+    }
     return once(std::move(out));
   }
 };
@@ -455,9 +465,9 @@ std::vector<at::Tensor> layer_norm(const at::Tensor& x, const std::optional<at::
   if (r.has_value()) r2 = rows_of(*r);
   if (w.has_value()) wf = w->to(at::kFloat).contiguous();
   if (b.has_value()) bf = b->to(at::kFloat).contiguous();
-  auto got = layer_norm_fwd(rows_of(x), r2, wf, bf, eps, out, 0, sum);
-  if (sum) return {std::get<0>(got).view(x.sizes()), std::get<1>(got).view(x.sizes())};
-  return {std::get<1>(got).view(x.sizes())};
+  auto got = layer_norm_fwd(rows_of(x), r2, wf, bf, eps, out, 0, sum, x.sizes());
+  if (sum) return {std::get<0>(got), std::get<1>(got)};
+  return {std::get<1>(got)};
 }
 std::vector<at::Tensor> layer_norm_autograd(const at::Tensor& x, const std::optional<at::Tensor>& r,
                                             const std::optional<at::Tensor>& w, const std::optional<at::Tensor>& b, double eps,

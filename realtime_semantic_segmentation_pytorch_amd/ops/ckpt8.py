@@ -4,7 +4,7 @@ What training holds between forward and backward is mostly activations.  A check
 them in a byte an element: 32 consecutive channels of a row share a power-of-two scale 2^e, the
 smallest with ``max|x| <= 127 * 2^e``, and an element is ``round(x / 2^e)`` (to nearest, ties to
 even), so a value is off by at most ``max|x| / 127`` of its block.  A block that holds an infinity or
-a NaN comes back as NaN.  Kernels: ``csrc/kernels/ckpt8.hip``, ``csrc/kernels/linear_ckpt8.hip``
+a NaN comes back as NaN.  Kernels: ``csrc/kernels/ckpt8.hip``, ``csrc/kernels/linear_ckpt8_*.hip``
 (format: ``csrc/include/rtseg_ckpt8.h``).
 
 * :func:`ckpt8_pack` / :func:`ckpt8_unpack`: a tensor to its checkpoint and back.

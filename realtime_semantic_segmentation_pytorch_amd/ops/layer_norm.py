@@ -1,4 +1,4 @@
-"""Layer norm over the last axis on the HIP kernels of ``csrc/kernels/layer_norm.hip``.
+"""Layer norm over the last axis on the HIP kernels of ``csrc/kernels/layer_norm_*.hip``.
 
 Reference: the Mix Transformer encoders that the reference reaches through
 segmentation_models_pytorch (reference models/__init__.py:67-81) normalise every token of the

@@ -1,4 +1,4 @@
-"""8-bit checkpoints and the checkpointing linear layer on the GPU (ckpt8.hip, linear_ckpt8.hip) against 64
+"""8-bit checkpoints and the checkpointing linear layer on the GPU (ckpt8.hip, linear_ckpt8_*.hip) against 64
 bits: codes, values and gradients, sizes around every tile edge, unaligned and strided operands, non-finite
 inputs, streams, captured graphs, and a Mix Transformer that trains on them."""
 import pytest
@@ -134,6 +134,21 @@ def test_linear_strided_and_unaligned(dtype):
         ref = LinearRef(x.reshape(50, 96), w, None, "gelu", dy.reshape(50, 64))
         check(a.grad.reshape(50, 96), ref.dx, ref.dx_tol, "dx")
         check(b.grad, ref.dw, ref.dw_tol, "dw")
+
+
+def test_linear_results_and_operands_changed_in_place():
+    x, w = _rand(2, 5, 64).requires_grad_(True), _rand(48, 64, seed=1).requires_grad_(True)
+    dy = _rand(2, 5, 48, seed=2)
+    want = torch.autograd.grad(ops.linear_ckpt8(x, w) * 2, (x, w), dy)
+    a = x * 1
+    y = ops.linear_ckpt8(a, w)
+    a.zero_()  # the checkpoint is of the values at the time
+    for g, t in zip(torch.autograd.grad(y.mul_(2), (w,), dy, retain_graph=True), want[1:]):
+        assert torch.equal(g, t)
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, (x,), dy)
 
 
 def test_linear_partial_gradients():

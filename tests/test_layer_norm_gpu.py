@@ -1,4 +1,4 @@
-"""Layer norm kernels (layer_norm.hip via ops.layer_norm) against 64 bits: values, the residual sum, the
+"""Layer norm kernels (layer_norm_*.hip via ops.layer_norm) against 64 bits: values, the residual sum, the
 gradients, the 8-bit checkpoint form; widths from one channel to the largest, unaligned and strided inputs,
 streams and captured graphs."""
 import pytest
@@ -81,6 +81,42 @@ def test_no_affine_large_mean_and_constant_rows():
     y = ops.layer_norm(x, eps=1e-6)
     y.sum().backward()
     assert not y.any() and torch.isfinite(x.grad).all()
+
+
+@pytest.mark.parametrize("c", [3, 45, 161, 2053, 4101])
+def test_no_affine_unaligned(c):
+    for ckpt in (False, True):
+        _run(13, c, F32, None, None, ckpt, affine=False)
+        _run(13, c, BF16, BF16, None, ckpt, affine=False)
+
+
+def test_leaves_of_one_type_keep_gradients_of_their_own():
+    x, r = (_rand(6, 32, seed=i).requires_grad_(True) for i in (1, 2))
+    for n in (1, 2):  # the second pass adds to what the first one left
+        s, y = ops.layer_norm(x, residual=r)
+        torch.autograd.backward([s, y], [torch.ones_like(s), _rand(6, 32, seed=3)])
+        if n == 1:
+            first = x.grad.clone()
+        assert torch.equal(x.grad, n * first) and torch.equal(r.grad, n * first)
+    assert x.grad.data_ptr() != r.grad.data_ptr()
+
+
+@pytest.mark.parametrize("shape", [(6, 32), (2, 3, 32)])
+def test_a_change_in_place_is_noticed(shape):
+    x = _rand(6, 32).view(shape).requires_grad_(True)
+    for ckpt in (False, True):
+        a = x * 1
+        y = ops.layer_norm(a, ckpt8=ckpt)
+        b = x * 1
+        s, z = ops.layer_norm(x, residual=b, ckpt8=ckpt)
+        a.add_(1)
+        s.add_(1)
+        for t in (y, z):
+            if ckpt:  # the checkpoint is of the values at the time
+                t.sum().backward()
+            else:
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    t.sum().backward()
 
 
 def test_rows_do_not_mix():
