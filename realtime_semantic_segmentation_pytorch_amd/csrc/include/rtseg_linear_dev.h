@@ -90,6 +90,29 @@ __device__ __forceinline__ uint2 pack8(const float* v) {
   }
 }
 
+// columns of a row of any alignment: W values from p on, of which n exist
+template <typename T, int W>
+__device__ __forceinline__ void put_any(T* p, int n, const float* v) {
+  constexpr int C = W % kPer16<T> == 0 ? kPer16<T> : 4;  // a store's
+  static_assert(W % C == 0, "whole stores");
+#pragma unroll
+  for (int e = 0; e < W; e += C) {
+    if (e + C <= n) {
+      if constexpr (C == kPer16<T>) {
+        const uint4 q = pack16<T>(v + e);
+        __builtin_memcpy(p + e, &q, 16);
+      } else {
+        const uint2 q = pack8<T>(v + e);
+        __builtin_memcpy(p + e, &q, 8);
+      }
+    } else {
+#pragma unroll
+      for (int i = e; i < e + C; ++i)
+        if (i < n) Io<T>::st(p + i, v[i]);
+    }
+  }
+}
+
 // largest of the chunk's absolute values as the bits of an fp32, NaN above infinity above every number
 template <typename T>
 __device__ __forceinline__ uint32_t top_bits(uint4 q, const float* v) {

@@ -53,6 +53,13 @@ __device__ __forceinline__ uint4 any16(const T* p, int64_t i, int64_t size) {
   if (last >= 0) __builtin_memcpy(&q, p + (i < last ? i : last), 16);
   return q;
 }
+// 16 bytes of any alignment that are all there
+template <typename T>
+__device__ __forceinline__ uint4 here16(const T* p, uint32_t i) {
+  uint4 q;
+  __builtin_memcpy(&q, p + i, 16);
+  return q;
+}
 template <typename T>
 __device__ __forceinline__ uint4 settle16(uint4 q, const T* p, int64_t i, int n) {
   if (n <= 0) return make_uint4(0u, 0u, 0u, 0u);

@@ -62,9 +62,18 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_dgrad_kernel(const
   for (int i = 0; i < XA; ++i)
     aoff[i] = (static_cast<uint32_t>(lrow + (WK == 1 ? NT / 8 * i : 0)) * p.R + lk + (WK == 1 ? 0 : NT / 8 * i / BM * BK)) * ES;
   uint4 ra[XA];
+  // unaligned rows: a step that the tensor has in whole is read as it lies, the others chunk by chunk
+  constexpr int ROWS = WK == 1 ? XA * NT / 8 : BM;
+  auto whole_a = [&](int m, int k0) { return static_cast<int64_t>(m) * BM + ROWS <= p.M && k0 + STEP <= p.R; };
+  auto whole_w = [&](int k0) { return n0 + BN <= p.N && k0 + STEP <= p.R; };
   auto fetch_a = [&](int m, int k0) {
     const int64_t skip = static_cast<int64_t>(m) * BM * p.R;
     const __amdgpu_buffer_rsrc_t ar = range(static_cast<const T*>(p.dy) + skip, (p.M * p.R - skip) * ES);
+    if (!VEC && whole_a(m, k0)) {
+#pragma unroll
+      for (int i = 0; i < XA; ++i) ra[i] = here16<T>(static_cast<const T*>(p.dy) + skip + k0, aoff[i] / ES);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < XA; ++i) {
       const int have = p.R - k0 - lk - (WK == 1 ? 0 : NT / 8 * i / BM * BK);
@@ -73,11 +82,12 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_dgrad_kernel(const
     }
   };
   auto stage_a = [&](int m, int k0, int buf) {
+    const bool ends = !VEC && !whole_a(m, k0);
 #pragma unroll
     for (int i = 0; i < XA; ++i) {
       const int slot = srow + NT / 8 * i, row = slot % BM;
       if (XA * NT > CH && slot >= WK * BM) break;
-      if constexpr (!VEC) {
+      if (ends) {
         const int64_t mm = static_cast<int64_t>(m) * BM + row;
         const int k = k0 + slot / BM * BK + chunk * PER;
         ra[i] = settle16<T>(ra[i], static_cast<const T*>(p.dy), mm * p.R + k, mm < p.M ? p.R - k : 0);
@@ -95,6 +105,12 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_dgrad_kernel(const
   auto fetch_w = [&](int k0) {
     const int64_t skip = static_cast<int64_t>(k0) * p.N;
     const __amdgpu_buffer_rsrc_t wr = range(W + skip, (wsize - skip) * ES);
+    if (!VEC && whole_w(k0)) {
+#pragma unroll
+      for (int i = 0; i < WB; ++i)
+        rw[i] = here16<T>(W + skip, static_cast<uint32_t>(wrow + WROWS * i) * p.N + wcol);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < WB; ++i) {
       const uint32_t turn = static_cast<uint32_t>(WROWS * i) * p.N;
@@ -104,11 +120,12 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_dgrad_kernel(const
     }
   };
   auto stage_w = [&](int k0, int buf) {
+    const bool ends = !VEC && !whole_w(k0);
 #pragma unroll
     for (int i = 0; i < WB; ++i) {
       const int row = wrow + WROWS * i;
       uint4 q = rw[i];
-      if constexpr (!VEC)
+      if (ends)
         q = settle16<T>(q, static_cast<const T*>(p.w), static_cast<int64_t>(k0 + row) * p.N + n0 + wcol, k0 + row < p.R ? whave : 0);
       if constexpr (ES == 2) {
         const int x = swz_w(row);  // bit 0 of the unit: the two halves change places
@@ -212,9 +229,7 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_dgrad_kernel(const
 #pragma unroll
         for (int e = 0; e < 16; e += PER) put16(orr, nc + e < p.N ? (row * p.N + nc + e) * ES : kOut, pack16<T>(v + e));
       } else if (m0 + row < p.M) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (nc + e < p.N) Io<T>::st(O + static_cast<int64_t>(row) * p.N + nc + e, v[e]);
+        put_any<T, 16>(O + static_cast<int64_t>(row) * p.N + nc, p.N - nc, v);
       }
     }
   };
@@ -314,19 +329,22 @@ void launch_cfg(DgradArgs p, hipStream_t st) {
   lin_dgrad_kernel<T, ACT, WN, WM, WK, TM, false, VEC, WAVES><<<grid, WN * WM * WK * 64, 0, st>>>(p);
 }
 
-// Tiles.  A problem of fewer than 256 tiles of 64 x 256 leaves CUs idle: 32 x 64 with the sum split four
-// ways.  Else narrow layers (N <= 64, 128) take their width and more rows, others 256 columns x 64 rows.
+// Tiles.  A problem of fewer than 256 tiles of 64 x 256 leaves CUs idle: 64 x 128 where those are 256 (4096 x 512
+// from 512 with gelu: 11.2 us against 15.8, one wave of four would work off the slopes), else 32 x 64 with the sum
+// split four ways.  Of the larger ones narrow layers (N <= 64, 128) take their width and more rows, others 256
+// columns x 64 rows.
 template <typename T, int ACT>
 void launch_dgrad(const DgradArgs& p, bool vec, hipStream_t st) {
   constexpr int F = sizeof(T) == 4 ? 1 : 0;  // fp32 holds more: fewer waves
   const int64_t tiles = (p.M + 63) / 64 * ((p.N + 255) / 256);
+  const bool mid = (p.M + 63) / 64 * ((p.N + 127) / 128) >= 256;
   if (!vec) {
-    if (tiles < 256) return launch_cfg<T, ACT, 1, 1, 4, 2, false, 2>(p, st);
+    if (tiles < 256 && !mid) return launch_cfg<T, ACT, 1, 1, 4, 2, false, 2>(p, st);
     return launch_cfg<T, ACT, 2, 2, 1, 2, false, 2>(p, st);
   }
-  if (tiles < 256) return launch_cfg<T, ACT, 1, 1, 4, 2, true, 3 - F>(p, st);
+  if (tiles < 256 && !mid) return launch_cfg<T, ACT, 1, 1, 4, 2, true, 3 - F>(p, st);
   if (p.N <= 64) return launch_cfg<T, ACT, 1, 4, 1, 2, true, 4 - F>(p, st);
-  if (p.N <= 128) return launch_cfg<T, ACT, 2, 2, 1, 2, true, 3>(p, st);
+  if (p.N <= 128 || tiles < 256) return launch_cfg<T, ACT, 2, 2, 1, 2, true, 3>(p, st);
   launch_cfg<T, ACT, 4, 1, 1, 4, true, 3 - F>(p, st);
 }
 

@@ -65,10 +65,19 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_fwd_kernel(const F
   for (int i = 0; i < XA; ++i)
     aoff[i] = (static_cast<uint32_t>(lrow + (WK == 1 ? NT / 8 * i : 0)) * p.K + lk + (WK == 1 ? 0 : NT / 8 * i / BM * BK)) * ES;
   uint4 ra[XA];
+  // unaligned rows: a step that the tensor has in whole is read as it lies, the others chunk by chunk
+  constexpr int ROWS = WK == 1 ? XA * NT / 8 : BM;
+  auto whole_a = [&](int m, int k0) { return static_cast<int64_t>(m) * BM + ROWS <= p.M && k0 + STEP <= p.K; };
+  auto whole_b = [&](int k0) { return n0 + BN <= p.N && k0 + STEP <= p.K; };
   auto fetch_a = [&](int m, int k0) {  // row tile m
     const int64_t skip = static_cast<int64_t>(m) * BM * p.K;
     const T* A = static_cast<const T*>(p.a) + skip;
     const __amdgpu_buffer_rsrc_t ar = range(A, (p.M * p.K - skip) * ES);
+    if (!VEC && whole_a(m, k0)) {
+#pragma unroll
+      for (int i = 0; i < XA; ++i) ra[i] = here16<T>(A + k0, aoff[i] / ES);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < XA; ++i) {
       const int have = p.K - k0 - lk - (WK == 1 ? 0 : NT / 8 * i / BM * BK);
@@ -91,12 +100,13 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_fwd_kernel(const F
     const int64_t m0 = static_cast<int64_t>(m) * BM;
     const __amdgpu_buffer_rsrc_t cr = range(p.codes + m0 * p.Cp, (p.M - m0) * p.Cp);
     const __amdgpu_buffer_rsrc_t er = range(p.scales + m0 * (p.Cp / kBlock), (p.M - m0) * (p.Cp / kBlock));
+    const bool ends = !VEC && !whole_a(m, k0);
 #pragma unroll
     for (int i = 0; i < XA; ++i) {
       const int slot = srow + NT / 8 * i, row = slot % BM;
       if (XA * NT > CH && slot >= WK * BM) break;
       const int k = k0 + slot / BM * BK + chunk * PER;
-      if constexpr (!VEC)
+      if (ends)
         ra[i] = settle16<T>(ra[i], static_cast<const T*>(p.a), (m0 + row) * p.K + k, m0 + row < p.M ? p.K - k : 0);
       {
         float v[PER];
@@ -139,6 +149,11 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_fwd_kernel(const F
   uint4 wf[2][TN];
   auto fetch_b = [&](int s, int k0) {
     const int kc = k0 + s * 4 * PER, have = p.K - kc - bk;
+    if (!VEC && whole_b(k0)) {
+#pragma unroll
+      for (int t = 0; t < TN; ++t) wf[s][t] = here16<T>(B + kc, boff[t] / ES);
+      return;
+    }
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
       if constexpr (VEC) wf[s][t] = buf16(br, have > 0 ? boff[t] : kOut, kc * ES);
@@ -163,7 +178,7 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_fwd_kernel(const F
       for (int j = 0; j < TN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   };
   auto multiply = [&](int s, int buf, int k0) {
-    if constexpr (!VEC) {
+    if (!VEC && !whole_b(k0)) {
       const int kc = k0 + s * 4 * PER, have = p.K - kc - bk;
 #pragma unroll
       for (int t = 0; t < TN; ++t)
@@ -200,9 +215,7 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_fwd_kernel(const F
           for (int e = 0; e < 4 * TN; e += 4) put8(orr, nc + e < p.N ? (row * p.N + nc + e) * ES : kOut, pack8<T>(v + e));
         }
       } else if (m0 + row < p.M) {
-#pragma unroll
-        for (int e = 0; e < 4 * TN; ++e)
-          if (nc + e < p.N) Io<T>::st(O + static_cast<int64_t>(row) * p.N + nc + e, v[e]);
+        put_any<T, 4 * TN>(O + static_cast<int64_t>(row) * p.N + nc, p.N - nc, v);
       }
     }
   };
@@ -292,7 +305,8 @@ void launch_cfg(FwdArgs p, hipStream_t st) {
   lin_fwd_kernel<T, ACT, WN, WM, WK, TM, TN, false, VEC, WAVES><<<grid, WN * WM * WK * 64, 0, st>>>(p);
 }
 
-// Tiles.  A problem of fewer than 256 tiles of 64 x 256 leaves CUs idle: 32 x 64 with k split four ways.
+// Tiles.  A problem of fewer than 256 tiles of 64 x 256 leaves CUs idle: 32 x 64 (fp32: 16 x 64) with k split four
+// ways.
 // Else narrow layers (N <= 64, 128) take their width and more rows, others 256 columns x 64 rows, and with
 // gelu all columns up to 512.
 template <typename T, int ACT>
@@ -300,10 +314,10 @@ void launch_fwd(const FwdArgs& p, bool vec, hipStream_t st) {
   constexpr int F = sizeof(T) == 4 ? 1 : 0;  // fp32 holds more: fewer waves
   const int64_t tiles = (p.M + 63) / 64 * ((p.N + 255) / 256);
   if (!vec) {
-    if (tiles < 256) return launch_cfg<T, ACT, 1, 1, 4, 2, 4, false, 3>(p, st);
-    return launch_cfg<T, ACT, 2, 2, 1, 2, 4, false, 3>(p, st);
+    if (tiles < 256) return launch_cfg<T, ACT, 1, 1, 4, 2 - F, 4, false, 3>(p, st);
+    return launch_cfg<T, ACT, 2, 2, 1, 2, 4, false, 3 - F>(p, st);
   }
-  if (tiles < 256) return launch_cfg<T, ACT, 1, 1, 4, 2, 4, true, 3>(p, st);
+  if (tiles < 256) return launch_cfg<T, ACT, 1, 1, 4, 2 - F, 4, true, 3>(p, st);
   if (p.N <= 64) return launch_cfg<T, ACT, 1, 4, 1, 2, 4, true, 3>(p, st);
   if (p.N <= 128) return launch_cfg<T, ACT, 2, 2, 1, 2, 4, true, 4 - F>(p, st);
   if constexpr (ACT == kCkptGelu) {

@@ -24,7 +24,7 @@ struct TnArgs {
   void* db;
   int64_t M, rows_per_split;
   int N, K, Cp, splits, ktiles, ntiles, w_dtype;
-  bool want_db, vo;     // vo: 4 consecutive k as one store
+  bool want_db;
 };
 
 __device__ __forceinline__ void put1(void* p, int dt, int64_t i, float v) {
@@ -33,10 +33,13 @@ __device__ __forceinline__ void put1(void* p, int dt, int64_t i, float v) {
   else static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);
 }
 
-__device__ __forceinline__ void put4(void* p, int dt, int64_t i, const float* v) {  // i is a multiple of 4
-  if (dt == kF32) *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
-  else if (dt == kBF16) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = pack8<uint16_t>(v);
-  else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = pack8<_Float16>(v);
+__device__ __forceinline__ void put4(void* p, int dt, int64_t i, const float* v) {  // of any alignment
+  if (dt == kF32) {
+    __builtin_memcpy(static_cast<float*>(p) + i, v, 16);
+  } else {
+    const uint2 q = dt == kBF16 ? pack8<uint16_t>(v) : pack8<_Float16>(v);
+    __builtin_memcpy(static_cast<uint16_t*>(p) + i, &q, 8);
+  }
 }
 
 // WN x WK waves of 16 TN columns n and 16 TK channels k each
@@ -71,6 +74,8 @@ __global__ void __launch_bounds__(WN* WK * 64, WAVES) lin_tn_kernel(const TnArgs
   const uint32_t zoff = static_cast<uint32_t>(zrow) * p.Cp + zcol, eoff = static_cast<uint32_t>(zrow) * ep + zcol / kBlock;
 
   uint4 yr[YN], zr[ZN];
+  // unaligned rows: a step that the tensor has in whole is read as it lies, the others chunk by chunk
+  auto whole = [&](int64_t m1) { return m1 + (YN / YG * YROWS > BS ? YN / YG * YROWS : BS) <= me && n0 + NB <= p.N; };
   uint8_t zb[ZN];
   auto fetch = [&](int64_t m1) {  // rows m1 .. m1 + BS - 1; those behind the split's last read 0
     const int64_t left = me - m1;
@@ -78,11 +83,13 @@ __global__ void __launch_bounds__(WN* WK * 64, WAVES) lin_tn_kernel(const TnArgs
     const __amdgpu_buffer_rsrc_t yb = range(Y, (left * p.N - n0) * ES);
     const __amdgpu_buffer_rsrc_t cb = range(p.codes + m1 * p.Cp + k0, left * p.Cp - k0);
     const __amdgpu_buffer_rsrc_t eb = range(p.scales + m1 * ep + k0 / kBlock, left * ep - k0 / kBlock);
+    const bool in = !VEC && whole(m1);
 #pragma unroll
     for (int i = 0; i < YN; ++i) {
       const int skip = i % YG * 8 * PER;  // columns
       const uint32_t o = yoff + static_cast<uint32_t>(i / YG * YROWS * ES) * p.N + skip * ES;
       if constexpr (VEC) yr[i] = buf16(yb, p.N - n0 - ycol - skip > 0 ? o : kOut);
+      else if (in) yr[i] = here16<T>(Y, o / ES);
       else yr[i] = any16<T>(static_cast<const T*>(p.dy), m1 * p.N + n0 + o / ES, p.M * p.N);
     }
 #pragma unroll
@@ -128,11 +135,12 @@ __global__ void __launch_bounds__(WN* WK * 64, WAVES) lin_tn_kernel(const TnArgs
 
   fetch(mb);
   for (int64_t m1 = mb; m1 < me; m1 += BS) {
+    const bool ends = !VEC && !whole(m1);
 #pragma unroll
     for (int i = 0; i < YN; ++i) {
       const int row = yrow + i / YG * YROWS, skip = i % YG * 8 * PER;
       if (YROWS > BS && row >= BS) break;
-      if constexpr (!VEC)
+      if (ends)
         yr[i] = settle16<T>(yr[i], static_cast<const T*>(p.dy), (m1 + row) * p.N + n0 + ycol + skip,
                             m1 + row < me ? p.N - n0 - ycol - skip : 0);
       ys[at(row, (tid & 7) + i % YG * 8, YR)] = yr[i];
@@ -215,8 +223,8 @@ __global__ void __launch_bounds__(WN* WK * 64, WAVES) lin_tn_kernel(const TnArgs
       float v[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = ES == 2 ? acc[i][j][e] : acc[(4 * i + e) % TK][j][(4 * i + e) / TK];
-      if (p.vo) {
-        if (k < p.K) put4(to, tt, base + k, v);
+      if (k + 4 <= p.K) {
+        put4(to, tt, base + k, v);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -235,29 +243,66 @@ __global__ void __launch_bounds__(WN* WK * 64, WAVES) lin_tn_kernel(const TnArgs
   }
 }
 
-// ws -> dw, db.  A block owns 32 elements, its 8 groups of 32 lanes every 8th split; the groups are added in
-// order: the same sum on every run, and 8 times the loads in flight of one thread an element.
-template <typename TW>
+// ws -> dw, db.  A block owns 256 / GR fours of elements, its GR groups of lanes every GR-th split; the groups
+// are added in order: the same sum on every run, and GR times the loads in flight of one thread a four.  Planes
+// that would be few blocks take 32 groups of 8 lanes: 128 x 128 from 128 splits in 3.7 us against 4.7, but 256 x 64
+// from 512, which is bound by its 34 MB, in 7.7 against 6.5.  (One element a lane took 9.5 us where 512 x 512 are joined
+// from 16 splits and 12.8 us for 320 x 1280 from 25: too many blocks.)
+template <typename TW, int GR>
 __global__ void __launch_bounds__(256) lin_wgrad_join_kernel(const float* __restrict__ ws, TW* dw, TW* db, int splits,
                                                              int64_t plane, int N) {
-  __shared__ float red[8][33];
-  const int el = threadIdx.x & 31, grp = threadIdx.x >> 5;
-  const int64_t e = blockIdx.x * static_cast<int64_t>(32) + el;
-  const bool is_w = e < plane, in = is_w || (e < plane + N && db != nullptr);
-  const float* src = is_w ? ws + e : ws + splits * plane + (e - plane);
+  constexpr int EL = 256 / GR;
+  __shared__ float4 red[GR][EL];
+  const int el = threadIdx.x % EL, grp = threadIdx.x / EL;
+  const int64_t q = blockIdx.x * static_cast<int64_t>(EL) + el, wq = (plane + 3) / 4;
+  const bool is_w = q < wq;
+  const int64_t e = 4 * (is_w ? q : q - wq), left = (is_w ? plane : db != nullptr ? N : 0) - e;
+  const float* src = ws + (is_w ? 0 : splits * plane) + e;
   const int64_t step = is_w ? plane : N;
-  float s = 0.f;
-  if (in) {
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float4& v) { s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w; };
+  if (left >= 4) {
 #pragma unroll 8
-    for (int i = grp; i < splits; i += 8) s += src[i * step];
+    for (int i = grp; i < splits; i += GR) {
+      float4 v;
+      __builtin_memcpy(&v, src + i * step, 16);
+      add(v);
+    }
+  } else if (left > 0) {
+    for (int i = grp; i < splits; i += GR)
+      add(make_float4(src[i * step], left > 1 ? src[i * step + 1] : 0.f, left > 2 ? src[i * step + 2] : 0.f, 0.f));
   }
   red[grp][el] = s;
   __syncthreads();
-  if (grp != 0 || !in) return;
+  if (grp != 0 || left <= 0) return;
 #pragma unroll
-  for (int q = 1; q < 8; ++q) s += red[q][el];
-  if (is_w) Io<TW>::st(dw + e, s);
-  else Io<TW>::st(db + (e - plane), s);
+  for (int i = 1; i < GR; ++i) add(red[i][el]);
+  TW* to = (is_w ? dw : db) + e;
+  const float v[4] = {s.x, s.y, s.z, s.w};
+  if (left >= 4) {
+    if constexpr (sizeof(TW) == 4) {
+      __builtin_memcpy(to, v, 16);
+    } else {
+      const uint2 o = pack8<TW>(v);
+      __builtin_memcpy(to, &o, 8);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < left) Io<TW>::st(to + i, v[i]);
+  }
+}
+
+void launch_join(int dtype, const float* ws, void* dw, void* db, int splits, int64_t plane, int N, hipStream_t st) {
+  const int64_t fours = (plane + 3) / 4 + (N + 3) / 4;
+  by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    auto go = [&](auto kernel, int64_t each) {
+      kernel<<<static_cast<unsigned>((fours + each - 1) / each), 256, 0, st>>>(ws, static_cast<T*>(dw), static_cast<T*>(db), splits, plane, N);
+    };
+    if (fours <= 512 * 32 && splits > 8 && splits <= 128) go(lin_wgrad_join_kernel<T, 32>, 8);
+    else go(lin_wgrad_join_kernel<T, 8>, 32);
+  });
 }
 
 // column sums of dy alone (a frozen weight with a trained bias): 64 columns x 4 row lanes a block, the
@@ -286,8 +331,10 @@ TnPlan tn_plan(int64_t M, int N, int K, int act) {
   w.cols = N <= 64 ? 64 : N <= 128 ? 128 : N <= 256 || act == kCkptNone ? 256 : N <= 320 ? 320 : 512;
   w.kt = w.cols >= 256 ? 64 : 128;
   const int64_t tiles = static_cast<int64_t>((N + w.cols - 1) / w.cols) * ((K + w.kt - 1) / w.kt);
-  int64_t s = 512 / tiles;                 // two blocks a CU
-  const int64_t most = (M + 255) / 256;    // of at least 256 rows each
+  // one block a CU; the second one of gelu hides its arithmetic (131072 x 256 x 64: 25.7 us against 31.5), without it
+  // it only doubles what is joined (131072 x 64 x 256 with its join: 21.8 us against 26.1)
+  int64_t s = (act == kCkptGelu ? 512 : 256) / tiles;
+  const int64_t most = (M + 127) / 128;    // of at least 128 rows each
   if (s > most) s = most;
   if (s < 1) s = 1;
   w.rows = ((M + s - 1) / s + 63) / 64 * 64;
@@ -330,7 +377,6 @@ void launch_lin_wgrad(const LinWgradArgs& a, hipStream_t st) {
   p.M = a.M; p.rows_per_split = w.rows; p.N = a.N; p.K = a.K; p.Cp = static_cast<int>(padded(a.K));
   p.splits = w.splits; p.w_dtype = a.w_dtype;
   p.want_db = a.db != nullptr;
-  p.vo = a.K % 4 == 0;
   const bool vec = a.N % (16 / elem(a.dtype)) == 0 && al16(a.dy);
   by_type(a.dtype, [&](auto t) {
     using T = decltype(t);
@@ -339,11 +385,7 @@ void launch_lin_wgrad(const LinWgradArgs& a, hipStream_t st) {
   });
   if (w.splits == 1) return;
   const int64_t plane = static_cast<int64_t>(a.N) * a.K;
-  const unsigned jg = static_cast<unsigned>((plane + a.N + 31) / 32);
-  by_type(a.w_dtype, [&](auto t) {
-    using T = decltype(t);
-    lin_wgrad_join_kernel<T><<<jg, 256, 0, st>>>(a.ws, static_cast<T*>(a.dw), static_cast<T*>(a.db), w.splits, plane, a.N);
-  });
+  launch_join(a.w_dtype, a.ws, a.dw, a.db, w.splits, plane, a.N, st);
 }
 
 int lin_colsum_splits(int64_t M) { return static_cast<int>(M < 64 ? 1 : (M / 64 < 512 ? M / 64 : 512)); }
@@ -356,10 +398,7 @@ void launch_lin_colsum(const void* dy, int dtype, float* ws, void* db, int db_dt
     using T = decltype(t);
     lin_colsum_kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(dy), ws, M, N, rows);
   });
-  by_type(db_dtype, [&](auto t) {
-    using T = decltype(t);
-    lin_wgrad_join_kernel<T><<<(N + 31) / 32, 256, 0, st>>>(ws, static_cast<T*>(nullptr), static_cast<T*>(db), splits, 0, N);
-  });
+  launch_join(db_dtype, ws, nullptr, db, splits, 0, N, st);
 }
 
 }  // namespace rtseg
