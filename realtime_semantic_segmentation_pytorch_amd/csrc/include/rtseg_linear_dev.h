@@ -156,7 +156,6 @@ __device__ __forceinline__ uint2 tr_read(const void* p) {
 // the 16 rows of a fragment read over the banks
 __device__ __forceinline__ int swz_a(int row) { return row & 7; }
 
-inline int elem(int dt) { return dt == kF32 ? 4 : 2; }
 template <class F>
 void by_type(int dt, F f) {
   if (dt == kF32) f(float{});

@@ -2,6 +2,8 @@
 // 16-byte aligned, from clamped addresses where they are not.
 #pragma once
 
+#include <type_traits>
+
 #include "rtseg_common.h"
 
 namespace rtseg {
@@ -40,6 +42,14 @@ __device__ __forceinline__ void put16(__amdgpu_buffer_rsrc_t r, uint32_t off, ui
 __device__ __forceinline__ void put8(__amdgpu_buffer_rsrc_t r, uint32_t off, uint2 v) {
   __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, v), r, static_cast<int>(off), 0, 0);
 }
+// A launch holds fewer than 2^32 threads: 2^24 - 1 blocks of 256.
+constexpr int64_t kMaxBlocks = (1 << 24) - 1;
+template <typename P>
+P* ahead(P* p, int64_t bytes) {  // null stays null
+  using Byte = std::conditional_t<std::is_const_v<P>, const char, char>;
+  return p == nullptr ? nullptr : reinterpret_cast<P*>(reinterpret_cast<Byte*>(p) + bytes);
+}
+inline int size_of(int dt) { return dt == kF32 ? 4 : 2; }
 inline bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Rows of any alignment.  The load is issued without a branch, from inside the tensor: p[i] where 16 bytes

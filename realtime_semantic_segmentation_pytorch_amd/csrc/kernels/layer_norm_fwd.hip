@@ -126,6 +126,22 @@ void launch_layer_norm_fwd(LnFwdArgs a, hipStream_t st) {
   a.lanes = p.lanes;
   const bool vec = a.C % 8 == 0 && al16(a.x) && al16(a.r) && al16(a.s) && al16(a.y) && al16(a.w) && al16(a.b);
   const int64_t rpb = kThreads / a.lanes;
+  if (a.rows > rpb * kMaxBlocks) {  // more than one launch holds
+    const int64_t rows = a.rows, first = rpb * kMaxBlocks / 64 * 64, n = first * a.C;
+    a.rows = first;
+    launch_layer_norm_fwd(a, st);
+    a.x = ahead(a.x, n * size_of(a.x_dtype));
+    a.r = ahead(a.r, n * size_of(a.r_dtype));
+    a.s = ahead(a.s, n * size_of(a.x_dtype));
+    a.y = ahead(a.y, n * size_of(a.y_dtype));
+    a.mean = ahead(a.mean, first * 4);
+    a.rstd = ahead(a.rstd, first * 4);
+    a.codes = ahead(a.codes, first * a.Cp);
+    a.scales = ahead(a.scales, first * (a.Cp / kBlock));
+    a.rows = rows - first;
+    launch_layer_norm_fwd(a, st);
+    return;
+  }
   const unsigned grid = static_cast<unsigned>((a.rows + rpb - 1) / rpb);
   by_types(a.x_dtype, a.y_dtype, [&](auto tx, auto to) {
     by_plan(p, [&](auto nv, auto block) {

@@ -354,10 +354,24 @@ void launch_dgrad(const DgradArgs& p, bool vec, hipStream_t st) {
 void launch_lin_dgrad(const LinDgradArgs& a, hipStream_t st) {
   using namespace lin;
   if (a.M == 0) return;
+  const int64_t most = kMaxBlocks / ((a.K + 63) / 64) * 16;  // rows of the smallest tiles that one launch holds
+  if (a.M > most) {
+    const int64_t cp = padded(a.K);
+    LinDgradArgs b = a;
+    b.M = most;
+    launch_lin_dgrad(b, st);
+    b.dy = ahead(a.dy, most * a.N * size_of(a.dtype));
+    b.dx = ahead(a.dx, most * a.K * size_of(a.dtype));
+    b.codes = ahead(a.codes, most * cp);
+    b.scales = ahead(a.scales, most * (cp / kBlock));
+    b.M = a.M - most;
+    launch_lin_dgrad(b, st);
+    return;
+  }
   DgradArgs p{};
   p.dy = a.dy; p.w = a.w; p.out = a.dx; p.codes = a.codes; p.scales = a.scales;
   p.M = a.M; p.N = a.K; p.R = a.N; p.Cp = static_cast<int>(padded(a.K));
-  const int per = 16 / elem(a.dtype);
+  const int per = 16 / size_of(a.dtype);
   p.vo = a.K % per == 0 && al16(a.dx);
   const bool vec = a.N % per == 0 && a.K % per == 0 && al16(a.dy) && al16(a.w);
   by_type(a.dtype, [&](auto t) {

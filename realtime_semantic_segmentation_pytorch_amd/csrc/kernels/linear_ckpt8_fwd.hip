@@ -333,10 +333,24 @@ void launch_fwd(const FwdArgs& p, bool vec, hipStream_t st) {
 void launch_lin_fwd(const LinFwdArgs& a, hipStream_t st) {
   using namespace lin;
   if (a.M == 0) return;
+  const int64_t most = kMaxBlocks / ((a.N + 63) / 64) * 16;  // rows of the smallest tiles that one launch holds
+  if (a.M > most) {
+    const int64_t cp = padded(a.K);
+    LinFwdArgs b = a;
+    b.M = most;
+    launch_lin_fwd(b, st);
+    b.x = ahead(a.x, most * a.K * size_of(a.dtype));
+    b.y = ahead(a.y, most * a.N * size_of(a.dtype));
+    b.codes = ahead(a.codes, most * cp);
+    b.scales = ahead(a.scales, most * (cp / kBlock));
+    b.M = a.M - most;
+    launch_lin_fwd(b, st);
+    return;
+  }
   FwdArgs p{};
   p.a = a.x; p.b = a.w; p.bias = a.b; p.out = a.y; p.codes = a.codes; p.scales = a.scales;
   p.M = a.M; p.N = a.N; p.K = a.K; p.Cp = static_cast<int>(padded(a.K));
-  const int per = 16 / elem(a.dtype);
+  const int per = 16 / size_of(a.dtype);
   p.vo = a.N % per == 0 && al16(a.y);
   p.bias_f32 = a.b_dtype == kF32;
   const bool vec = a.K % per == 0 && al16(a.x) && al16(a.w);

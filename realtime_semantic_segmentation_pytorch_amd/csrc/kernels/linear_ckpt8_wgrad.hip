@@ -377,7 +377,7 @@ void launch_lin_wgrad(const LinWgradArgs& a, hipStream_t st) {
   p.M = a.M; p.rows_per_split = w.rows; p.N = a.N; p.K = a.K; p.Cp = static_cast<int>(padded(a.K));
   p.splits = w.splits; p.w_dtype = a.w_dtype;
   p.want_db = a.db != nullptr;
-  const bool vec = a.N % (16 / elem(a.dtype)) == 0 && al16(a.dy);
+  const bool vec = a.N % (16 / size_of(a.dtype)) == 0 && al16(a.dy);
   by_type(a.dtype, [&](auto t) {
     using T = decltype(t);
     if (a.act == kCkptGelu) launch_tn<T, kCkptGelu>(p, w, vec, st);

@@ -79,3 +79,51 @@ def test_linear():
     assert not _middle(x.grad).any()
     check(w.grad, ref.dw, ref.dw_tol, "dw")
     check(b.grad, ref.db, ref.db_tol, "db")
+
+
+# ------------------------------------------------------------------------------- more blocks than a launch holds
+
+
+def _rows(rows, cut):
+    return torch.cat([torch.arange(20), torch.arange(cut - 20, cut + 20), torch.arange(rows - 20, rows)]).cuda()
+
+
+def test_layer_norm_of_more_rows_than_one_launch_holds():
+    c, cut = 512, 4 * (2 ** 24 - 1) // 64 * 64  # 4 rows a block
+    rows = cut + 777
+    if torch.cuda.mem_get_info()[0] < 190 << 30:
+        pytest.skip("needs 190 GB of device memory")
+    at = _rows(rows, cut)
+    x0, dy0 = _rand(len(at), c, 0), _rand(len(at), c, 1)
+    w, b = (torch.rand(c, generator=torch.Generator().manual_seed(s)).cuda().requires_grad_(True) for s in (2, 3))
+    ref = NormRef(x0, w, b, 1e-5, None, BF16, dy0, None, True)
+    x = torch.zeros(rows, c, device="cuda", dtype=BF16)
+    x[at] = x0
+    y = ops.layer_norm(x, w, b, ckpt8=True)
+    del x
+    check(y[at], ref.y, ref.y_tol, "y")
+    dy = torch.zeros_like(y)
+    dy[at] = dy0
+    y.backward(dy)
+    check(w.grad, ref.dw, ref.dw_tol, "dw")
+    check(b.grad, ref.db, ref.db_tol, "db")
+
+
+@pytest.mark.parametrize("k,n", [(64, 2 ** 20), (2 ** 20, 8)])
+def test_linear_of_more_tiles_than_one_launch_holds(k, n):
+    cut = (2 ** 24 - 1) // 2 ** 14 * 16
+    rows = cut + 777
+    at = _rows(rows, cut)
+    x0, dy0 = _rand(len(at), k, 0), _rand(len(at), n, 1)
+    w = (_rand(n, k, 2) / 8).requires_grad_(True)
+    x = torch.zeros(rows, k, device="cuda", dtype=BF16)
+    x[at] = x0
+    x.requires_grad_(True)
+    y = ops.linear_ckpt8(x, w, None, act="gelu")
+    dy = torch.zeros_like(y)
+    dy[at] = dy0
+    y.backward(dy)
+    ref = LinearRef(x0, w, None, "gelu", dy0)
+    check(y[at], ref.y, ref.y_tol, "y")
+    check(x.grad[at], ref.dx, ref.dx_tol, "dx")
+    check(w.grad, ref.dw, ref.dw_tol, "dw")
