@@ -8,7 +8,9 @@
 //
 // What bounds it: HBM and, with gelu, the VALU work of decoding.  So a tile is as wide in n as the layer
 // (up to 512), which decodes every code once, and 64 or 128 channels of k; the number of blocks is held near
-// two a CU, because each of them writes (and the join reads) one fp32 tile.
+// one or two a CU, because each of them writes (and the join reads) one fp32 tile.  Measured with the join:
+// 131072 rows of 256 x 64 21.8 us (76 MB, 3.5 TB/s), of 64 x 256 with gelu 29.8 us, 32768 of 320 x 1280 with gelu
+// 74 us (363 TF).
 #include "rtseg_linear_dev.h"
 
 namespace rtseg {
