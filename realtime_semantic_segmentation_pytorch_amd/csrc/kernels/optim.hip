@@ -28,6 +28,14 @@ namespace {
 constexpr int kOptBlock = 256;
 constexpr int kOptUnroll = 4;
 
+// A product as rounded: not fused into the sum behind it.  Which products the compiler fuses depends on the
+// target's features; torch's optimizers scale a state in place (one rounding) and then add to it, and a
+// training run that follows theirs step by step has to round where they do.
+__device__ __forceinline__ float rounded(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
 // torch.lerp's two-sided formula (exact endpoint at w = 1).
 __device__ __forceinline__ float lerp_like_torch(float a, float b, float w) {
   return w < 0.5f ? a + w * (b - a) : b - (b - a) * (1.f - w);
@@ -85,22 +93,22 @@ __global__ void __launch_bounds__(kOptBlock) fused_opt_kernel(const int64_t* met
       float pp = pv[u];
       float g = gv[u] * hp.grad_scale;
       if (sgd) {
-        if (hp.weight_decay != 0.f) g += hp.weight_decay * pp;
+        if (hp.weight_decay != 0.f) g = __builtin_fmaf(hp.weight_decay, pp, g);
         float d = g;
         if (hp.momentum != 0.f) {
-          const float b = first ? g : hp.momentum * av[u] + (1.f - hp.dampening) * g;
+          const float b = first ? g : rounded(hp.momentum * av[u]) + rounded((1.f - hp.dampening) * g);
           m1[i] = b;
-          d = hp.nesterov ? g + hp.momentum * b : b;
+          d = hp.nesterov ? __builtin_fmaf(hp.momentum, b, g) : b;
         }
-        pp -= hp.lr * d;
+        pp = __builtin_fmaf(-hp.lr, d, pp);
       } else {
         if (hp.mode == kOptAdamW) pp *= 1.f - hp.lr * hp.weight_decay;
-        else if (hp.weight_decay != 0.f) g += hp.weight_decay * pp;
-        const float m = hp.beta1 * av[u] + (1.f - hp.beta1) * g;
-        const float v = hp.beta2 * bv[u] + (1.f - hp.beta2) * g * g;
+        else if (hp.weight_decay != 0.f) g = __builtin_fmaf(hp.weight_decay, pp, g);
+        const float m = __builtin_fmaf(hp.beta1, av[u], (1.f - hp.beta1) * g);
+        const float v = rounded(hp.beta2 * bv[u]) + rounded((1.f - hp.beta2) * g * g);
         m1[i] = m;
         m2[i] = v;
-        const float denom = sqrtf(v) * hp.inv_sqrt_bc2 + hp.eps;
+        const float denom = rounded(sqrtf(v) * hp.inv_sqrt_bc2) + hp.eps;
         pp -= hp.step_size * m / denom;
       }
       p[i] = pp;
