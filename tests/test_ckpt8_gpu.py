@@ -151,6 +151,26 @@ def test_linear_results_and_operands_changed_in_place():
         torch.autograd.grad(y, (x,), dy)
 
 
+@pytest.mark.parametrize("lead", [(), (0, 5), (2, 0), (1, 1, 3)])
+def test_token_ops_leading_axes(lead):
+    x, w = _rand(*lead, 64).requires_grad_(True), _rand(48, 64, seed=1).requires_grad_(True)
+    y = ops.linear_ckpt8(x, w, act="gelu")
+    s, z = ops.layer_norm(x, residual=x, ckpt8=True)  # one tensor twice: its gradients add up
+    assert y.shape == (*lead, 48) and s.shape == z.shape == x.shape
+    one = x.detach().reshape(-1, 64).requires_grad_(True)
+    s1, z1 = ops.layer_norm(one, residual=one, ckpt8=True)
+    y1 = ops.linear_ckpt8(one, w, act="gelu")
+    for out, out1, leaves, leaves1 in ((y, y1, (x, w), (one, w)), (z, z1, (x,), (one,))):  # apart: sums of three round in an order
+        dy = _rand(*out.shape, seed=2)
+        got = torch.autograd.grad(out, leaves, dy)
+        want = torch.autograd.grad(out1, leaves1, dy.reshape(out1.shape))
+        assert all(torch.equal(p.reshape(q.shape), q) for p, q in zip(got, want))
+    assert torch.equal(y.reshape(y1.shape), y1)
+    assert torch.equal(s.reshape(-1, 64), s1) and torch.equal(z.reshape(-1, 64), z1)
+    c = ops.ckpt8_pack(x.detach())
+    assert torch.equal(ops.ckpt8_unpack(c).reshape(-1, 64), ops.ckpt8_unpack(ops.ckpt8_pack(one.detach())))
+
+
 def test_linear_partial_gradients():
     leaves = {"x": _rand(200, 96, dtype=BF16), "w": _rand(40, 96, seed=1), "b": _rand(40, seed=2)}
     dy = _rand(200, 40, seed=3, dtype=BF16)
