@@ -369,6 +369,19 @@ def test_mit_trains_on_checkpoints_and_holds_less():
     assert hb < 0.75 * ha, (ha, hb)
 
 
+def _check_replay(got, want):
+    """Parameter gradients of two runs of one step.  The library's data gradient of a patch embedding is not the same
+    fp32 bits on every run (1e-7, also with the stock layers; every forward is), and where its rounding to bf16 falls on
+    the other side a gradient element moves by 2^-8 of itself.  2e-2 is five such roundings in a row, all of them and all
+    in one direction.  The mean square of a layer norm's output has no gradient in front of the norm: dy = c h, and
+    g - mean(g) - h mean(g h) = c h (1 - mean(h^2)) = 0, so what the parameters there get is the residue of the
+    roundings, 2^-8 of what comes in, for which no bound relative to itself holds: it is held to 2e-2 of 2^-8 of the
+    whole gradient."""
+    total = float(torch.stack([b.norm() for b in want]).norm())
+    for a, b in zip(got, want):
+        assert float((a - b).norm()) <= 2e-2 * max(float(b.norm()), 2.0 ** -8 * total)
+
+
 @pytest.mark.no_guard
 def test_mit_checkpoint_step_as_a_graph():
     x = _rand(2, 3, 64, 64).contiguous(memory_format=torch.channels_last)
@@ -394,6 +407,34 @@ def test_mit_checkpoint_step_as_a_graph():
         x.copy_(_rand(*x.shape, seed=turn))
         g.replay()
         eager = step()
-        # MIOpen's and attention's own backward need not be the same bits run to run: compare as fp32 sums of bf16 products
-        assert all(_rel(a, b) < 2e-2 or float(b.norm()) < 1e-6 for a, b in zip(out, eager))
+        _check_replay(out, eager)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.no_guard
+def test_mit_checkpoint_step_as_a_graph_with_a_weighted_loss():
+    x = _rand(2, 3, 64, 64).contiguous(memory_format=torch.channels_last)
+    enc = _mit(act_ckpt8=True).encoder
+    params = [p for n, p in enc.named_parameters() if not n.startswith("head.")]
+    with torch.no_grad():
+        weigh = [_rand(*f.shape, seed=50 + i) for i, f in enumerate(enc(x)[2:])]
+
+    def step():
+        with torch.autocast("cuda", dtype=BF16, cache_enabled=False):
+            loss = sum((f.float() * r).mean() for f, r in zip(enc(x)[2:], weigh))
+        return torch.autograd.grad(loss, params)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for turn in range(4):
+        x.copy_(_rand(*x.shape, seed=turn))
+        g.replay()
+        _check_replay(out, step())
         torch.cuda.synchronize()
