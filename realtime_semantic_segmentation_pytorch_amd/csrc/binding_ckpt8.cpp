@@ -21,9 +21,9 @@ constexpr int64_t kBlock = 32;
 constexpr int64_t kMaxChannels = 1 << 20;  // the kernels' tile counts along channels are grid.y / int
 int64_t padded(int64_t c) { return (c + kBlock - 1) / kBlock * kBlock; }
 
-bool float_type(const at::Tensor& t) {
-  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf;
-}
+bool float_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+bool float_type(const at::Tensor& t) { return float_type(t.scalar_type()); }
+int type_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : 2; }
 
 // contiguous fp32 / bf16 / fp16 [rows, C] on the GPU
 void check_rows(const at::Tensor& t, const char* op, const char* what) {
@@ -71,17 +71,18 @@ std::tuple<at::Tensor, at::Tensor> ckpt8_pack(const at::Tensor& x) {
   return {codes, scales};
 }
 
-at::Tensor ckpt8_unpack(const at::Tensor& codes, const at::Tensor& scales, int64_t C, at::ScalarType dtype) {
+// held: the type of the tensor that was packed
+at::Tensor ckpt8_unpack(const at::Tensor& codes, const at::Tensor& scales, int64_t C, at::ScalarType dtype, at::ScalarType held) {
   TORCH_CHECK(codes.dim() == 2 && C >= 1 && C <= kMaxChannels,
               "rtseg.ckpt8_unpack: codes must be [rows, padded channels] with 1 .. ", kMaxChannels, " channels");
   TORCH_CHECK(codes.size(0) < std::numeric_limits<int>::max(), "rtseg.ckpt8_unpack: too many rows");
   check_ckpt(codes, scales, codes.size(0), C, codes, "ckpt8_unpack");
-  TORCH_CHECK(dtype == at::kFloat || dtype == at::kBFloat16 || dtype == at::kHalf,
-              "rtseg.ckpt8_unpack: fp32, bf16 or fp16 expected, got ", dtype);
+  for (const at::ScalarType t : {dtype, held})
+    TORCH_CHECK(float_type(t), "rtseg.ckpt8_unpack: fp32, bf16 or fp16 expected, got ", t);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
   at::Tensor x = at::empty({codes.size(0), C}, codes.options().dtype(dtype));
-  launch_ckpt8_unpack(codes.data_ptr<int8_t>(), scales.data_ptr<uint8_t>(), x.data_ptr(), dtype_code(x), x.size(0),
-                      static_cast<int>(C), cur_stream());
+  launch_ckpt8_unpack(codes.data_ptr<int8_t>(), scales.data_ptr<uint8_t>(), x.data_ptr(), dtype_code(x), type_code(held),
+                      x.size(0), static_cast<int>(C), cur_stream());
   return x;
 }
 
@@ -486,7 +487,7 @@ std::vector<at::Tensor> layer_norm_autograd(const at::Tensor& x, const std::opti
 
 TORCH_LIBRARY_FRAGMENT(rtseg, m) {
   m.def("ckpt8_pack(Tensor x) -> (Tensor, Tensor)");
-  m.def("ckpt8_unpack(Tensor codes, Tensor scales, int channels, ScalarType dtype) -> Tensor");
+  m.def("ckpt8_unpack(Tensor codes, Tensor scales, int channels, ScalarType dtype, ScalarType held) -> Tensor");
   // -> [y], or [x + r, y] with sum
   m.def("layer_norm(Tensor x, Tensor? r, Tensor? w, Tensor? b, float eps, ScalarType out, bool ckpt8, bool sum) -> Tensor[]");
   m.def("linear_ckpt8(Tensor x, Tensor w, Tensor? b, int act) -> Tensor");

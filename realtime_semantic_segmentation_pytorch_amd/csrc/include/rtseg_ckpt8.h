@@ -4,8 +4,10 @@
 // C are 0) and one scale byte per block of 32 consecutive channels of a row, [rows, Cp / 32]:
 //     e = the smallest integer >= -126 with max |x| <= 127 * 2^e,   q = rne(x / 2^e),   byte = e + 127.
 // The scale is a power of two, so dividing by it is exact (one rounding in all, at most half of 2^e)
-// and q * 2^e fits bf16 / fp16 / fp32 exactly wherever 2^e does: a matrix product reads the checkpoint
-// through bf16 MFMA with no further rounding.  A block that holds an infinity or a NaN gets the scale
+// and q * 2^e fits the type of the tensor exactly: a matrix product reads the checkpoint through bf16
+// MFMA with no further rounding.  The one value that does not fit is 64 * 2^e of the type's largest
+// scale, which what lies in the last half step below infinity rounds up to: it decodes to the type's
+// largest finite value, which is nearer still to what was packed (`hold`).  A block that holds an infinity or a NaN gets the scale
 // byte 255 and codes 0, which decode to 0 * inf = NaN: an overflowed activation still shows in the
 // gradients that are computed from it (the loss scaler of fp16 training looks for exactly that).
 #pragma once
@@ -48,6 +50,22 @@ __device__ __forceinline__ uint32_t code4(const float* v, float inv, bool bad) {
 __device__ __forceinline__ void decode4(uint32_t w, float scale, float* v) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(static_cast<int8_t>(w >> (8 * i))) * scale;
+}
+
+// The last scale byte of T's blocks, and the largest finite value: max = f * 2^(byte - 127) with f in (63.5, 64).
+template <typename T>
+constexpr uint32_t kTopByte = __is_same(T, _Float16) ? 137u : 249u;
+template <typename T>
+constexpr uint32_t kTopBits = __is_same(T, _Float16) ? 0x477fe000u : sizeof(T) == 2 ? 0x7f7f0000u : 0x7f7fffffu;
+// N values that were decoded with this scale byte, held in T's range.  A branch and not a clamp of each value: next to
+// no block takes it, and its values are numbers (a NaN would be clamped to one).
+template <typename T, int N>
+__device__ __forceinline__ void hold(uint32_t byte, float* v) {
+  if (byte == kTopByte<T>) {
+    const float top = __uint_as_float(kTopBits<T>);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = fminf(fmaxf(v[i], -top), top);
+  }
 }
 
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {  // over 4 consecutive lanes

@@ -438,7 +438,8 @@ void launch_shuffle(const Tensor4& in, const Tensor4& out, int mode, int r, bool
 // 8-bit activation checkpoints (format: rtseg_ckpt8.h): x [rows, C] contiguous fp32 / bf16 / fp16,
 // codes int8 [rows, Cp], scales uint8 [rows, Cp / 32], Cp = C rounded up to 32; codes 8-byte aligned.
 void launch_ckpt8_pack(const void* x, int dtype, int8_t* codes, uint8_t* scales, int64_t rows, int C, hipStream_t st);
-void launch_ckpt8_unpack(const int8_t* codes, const uint8_t* scales, void* x, int dtype, int64_t rows, int C,
+// held: the type of the tensor that was packed
+void launch_ckpt8_unpack(const int8_t* codes, const uint8_t* scales, void* x, int dtype, int held, int64_t rows, int C,
                          hipStream_t st);
 
 // ---- layer_norm_*.hip ---------------------------------------------------------------

@@ -47,7 +47,8 @@ __global__ void __launch_bounds__(256) ckpt8_pack_kernel(const T* __restrict__ x
   }
 }
 
-template <typename T, bool VEC>
+// H: the type of the tensor that was packed
+template <typename T, typename H, bool VEC>
 __global__ void __launch_bounds__(256) ckpt8_unpack_kernel(const uint2* __restrict__ codes,
                                                            const uint8_t* __restrict__ scales, T* __restrict__ x,
                                                            int64_t items, int64_t rows, int C, int items_row) {
@@ -56,10 +57,12 @@ __global__ void __launch_bounds__(256) ckpt8_unpack_kernel(const uint2* __restri
     const int64_t row = it / items_row;
     const int c = static_cast<int>(it - row * items_row) * 8;
     const uint2 w = codes[it];
-    const float s = scale_of(scales[it >> 2]);
+    const uint32_t byte = scales[it >> 2];
+    const float s = scale_of(byte);
     float v[8];
     decode4(w.x, s, v);
     decode4(w.y, s, v + 4);
+    hold<H, 8>(byte, v);
     const Raw8<T> r = raw8<T>(v);
     if constexpr (VEC) {
       if (c < C) {
@@ -99,7 +102,7 @@ void launch_ckpt8_pack(const void* x, int dtype, int8_t* codes, uint8_t* scales,
   });
 }
 
-void launch_ckpt8_unpack(const int8_t* codes, const uint8_t* scales, void* x, int dtype, int64_t rows, int C,
+void launch_ckpt8_unpack(const int8_t* codes, const uint8_t* scales, void* x, int dtype, int held, int64_t rows, int C,
                          hipStream_t st) {
   const int per = static_cast<int>(padded(C) / 8);
   const int64_t items = rows * per;
@@ -107,8 +110,12 @@ void launch_ckpt8_unpack(const int8_t* codes, const uint8_t* scales, void* x, in
   const int grid = stream_grid(items, 256);
   by_rows(dtype, x, C, [&](auto t, auto vec) {
     using T = decltype(t);
-    constexpr auto kernel = &ckpt8_unpack_kernel<T, decltype(vec)::value>;
-    kernel<<<grid, 256, 0, st>>>(reinterpret_cast<const uint2*>(codes), scales, static_cast<T*>(x), items, rows, C, per);
+    auto go = [&](auto kernel) {
+      kernel<<<grid, 256, 0, st>>>(reinterpret_cast<const uint2*>(codes), scales, static_cast<T*>(x), items, rows, C, per);
+    };
+    if (held == kF32) go(&ckpt8_unpack_kernel<T, float, decltype(vec)::value>);
+    else if (held == kBF16) go(&ckpt8_unpack_kernel<T, uint16_t, decltype(vec)::value>);
+    else go(&ckpt8_unpack_kernel<T, _Float16, decltype(vec)::value>);
   });
 }
 

@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(kThreads, bwd_blocks_cu(NV) - (VEC ? 0 : 1)) l
         const float s = scale_of(scale[j]);
         decode4(codes[j].x, s, v);
         decode4(codes[j].y, s, v + 4);
+        hold<TX, 8>(scale[j], v);
       } else {
         xs.settle(xr[j], e[j], n);
         unraw8<TX>(xr[j], v);

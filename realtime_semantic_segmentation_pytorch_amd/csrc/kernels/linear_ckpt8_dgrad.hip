@@ -219,13 +219,12 @@ __global__ void __launch_bounds__(WN* WM* WK * 64, WAVES) lin_dgrad_kernel(const
       if constexpr (ACT == kCkptGelu) {
         const float sc = scale_of(cb[i]);
         const uint32_t w4[4] = {cw[i].x, cw[i].y, cw[i].z, cw[i].w};
+        float z[16];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float z[4];
-          decode4(w4[j], sc, z);
+        for (int j = 0; j < 4; ++j) decode4(w4[j], sc, z + 4 * j);
+        hold<T, 16>(cb[i], z);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[4 * j + e] *= gelu_slope<T>(z[e]);
-        }
+        for (int e = 0; e < 16; ++e) v[e] *= gelu_slope<T>(z[e]);
       }
       if (p.vo) {
 #pragma unroll

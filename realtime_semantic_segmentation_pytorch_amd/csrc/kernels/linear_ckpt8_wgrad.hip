@@ -156,6 +156,7 @@ __global__ void __launch_bounds__(WN* WK * 64, WAVES) lin_tn_kernel(const TnArgs
       float v[16];
 #pragma unroll
       for (int q = 0; q < 4; ++q) decode4(w4[q], sc, v + 4 * q);
+      hold<T, 16>(zb[i], v);
       if constexpr (ACT == kCkptGelu) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = gelu<T>(v[e]);

@@ -3,7 +3,8 @@
 What training holds between forward and backward is mostly activations.  A checkpoint holds one of
 them in a byte an element: 32 consecutive channels of a row share a power-of-two scale 2^e, the
 smallest with ``max|x| <= 127 * 2^e``, and an element is ``round(x / 2^e)`` (to nearest, ties to
-even), so a value is off by at most ``max|x| / 127`` of its block.  A block that holds an infinity or
+even), so a value is off by at most ``max|x| / 127`` of its block.  (What the last half step of a type's
+range rounds up to, the type does not hold: it comes back as the largest finite value.)  A block that holds an infinity or
 a NaN comes back as NaN.  Kernels: ``csrc/kernels/ckpt8.hip``, ``csrc/kernels/linear_ckpt8_*.hip``
 (format: ``csrc/include/rtseg_ckpt8.h``).
 
@@ -63,10 +64,12 @@ def _pack_reference(x2: torch.Tensor):
     return q.to(torch.int8).view(rows, cp), scales.to(torch.uint8)
 
 
-def _unpack_reference(codes, scales, c, dtype):
+def _unpack_reference(codes, scales, c, dtype, held=torch.float32):
+    """``held``: the type of the tensor that was packed."""
     s = torch.ldexp(torch.ones_like(scales, dtype=torch.float32), scales.to(torch.int32) - 127)
     s = torch.where(scales == 255, torch.full_like(s, float("nan")), s)
     v = codes.float().view(*scales.shape, BLOCK) * s.unsqueeze(-1)
+    v = v.clamp(torch.finfo(held).min, torch.finfo(held).max)  # NaN stays NaN
     return v.view(codes.shape)[:, :c].to(dtype)
 
 
@@ -93,7 +96,7 @@ def ckpt8_unpack(ckpt: Ckpt8, dtype: Optional[torch.dtype] = None) -> torch.Tens
         raise TypeError(f"ckpt8_unpack: fp32, bf16 or fp16 expected, got {dtype}")
     c = ckpt.shape[-1]
     f = ops().ckpt8_unpack if use_hip(ckpt.codes, "ckpt8") else _unpack_reference
-    return f(ckpt.codes, ckpt.scales, c, dtype).view(ckpt.shape)
+    return f(ckpt.codes, ckpt.scales, c, dtype, ckpt.dtype).view(ckpt.shape)
 
 
 @contextlib.contextmanager
@@ -130,6 +133,11 @@ def ckpt8_saved(x: Optional[torch.Tensor]):
 # ---------------------------------------------------------------------------------- linear
 
 
+def _gelu(v):
+    """The erf form in an order that holds at the largest values (2 v is not formed)."""
+    return 0.5 * v * (1 + torch.erf(v * math.sqrt(0.5)))
+
+
 def _gelu_slope(z):
     return 0.5 * (1 + torch.erf(z * math.sqrt(0.5))) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
 
@@ -137,7 +145,7 @@ def _gelu_slope(z):
 def linear_ckpt8_reference(x2, weight, bias, act):
     """Forward of :func:`linear_ckpt8` in PyTorch: the activation rounded to ``x``'s type, the product
     and its operands in that type."""
-    a = F.gelu(x2.float()).to(x2.dtype) if act == "gelu" else x2
+    a = _gelu(x2.float()).to(x2.dtype) if act == "gelu" else x2
     with torch.autocast(x2.device.type, enabled=False):
         return F.linear(a, weight.to(x2.dtype), None if bias is None else bias.to(x2.dtype))
 
@@ -160,13 +168,13 @@ class _LinearCkpt8Fn(torch.autograd.Function):
         codes, scales, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = dw = db = None
-        z = None if codes is None else _unpack_reference(codes, scales, ctx.k, torch.float32)
+        z = None if codes is None else _unpack_reference(codes, scales, ctx.k, torch.float32, dy.dtype)
         g = dy.float()
         if need_x:
             dx = g @ weight.to(dy.dtype).float()
             dx = (dx * _gelu_slope(z) if ctx.act == "gelu" else dx).to(dy.dtype)
         if need_w:
-            a = F.gelu(z).to(dy.dtype).float() if ctx.act == "gelu" else z
+            a = _gelu(z).to(dy.dtype).float() if ctx.act == "gelu" else z
             dw = (g.t() @ a).to(ctx.wtype)
         if need_b:
             db = g.sum(0).to(ctx.wtype)

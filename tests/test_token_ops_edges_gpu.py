@@ -1,0 +1,95 @@
+"""Layer norm, 8-bit checkpoints and the checkpointing linear layer on the GPU at the edges of their types and of
+their contracts."""
+import pytest
+import torch
+
+import _token_ops
+from _token_ops import LinearRef, NormRef, check
+from realtime_semantic_segmentation_pytorch_amd import ops
+from realtime_semantic_segmentation_pytorch_amd.ops.ckpt8 import _pack_reference
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+DTYPES = [F32, BF16, F16]
+
+
+@pytest.fixture(autouse=True)
+def _lib():
+    assert ops.load(), "HIP extension must load on the GPU box"
+
+
+def _rand(*shape, seed=0, dtype=F32, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to("cuda", dtype)
+
+
+# ------------------------------------------------------------------------------- the top of the range
+
+_blocks = _token_ops.checkpoint
+
+
+def _held(x, dtype=None):
+    """The checkpoint's values in fp64: what its blocks round to, and no more than x's type (or ``dtype``) holds."""
+    top = torch.finfo(dtype or x.dtype).max
+    return _blocks(x).clamp(-top, top)
+
+
+def _top_rows(rows, c, dtype, top=1.0):
+    """Normal values; some rows with one of the largest of the type, or in the last half step below them."""
+    x = _rand(rows, c, dtype=dtype)
+    big = torch.finfo(dtype).max
+    for row, v in ((1, big), (2, -big), (4, big * 0.9945), (5, -big * 0.993), (7, big * 0.99)):
+        x[row, (7 * row) % c] = v * top
+    return x
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [64, 45])
+def test_the_largest_values_come_back_finite(dtype, c):
+    x = _top_rows(20, c, dtype)
+    p = ops.ckpt8_pack(x)
+    codes, scales = _pack_reference(x.cpu())
+    assert torch.equal(p.codes.cpu(), codes) and torch.equal(p.scales.cpu(), scales)
+    v = ops.ckpt8_unpack(p)
+    assert torch.isfinite(v).all() and torch.equal(v.double(), _held(x))
+    amax = x.double().abs().amax(1, keepdim=True)
+    assert ((v.double() - x.double()).abs() <= amax / 127).all()
+    for t in DTYPES:  # the values that the checkpoint stands for, rounded once
+        assert torch.equal(ops.ckpt8_unpack(p, t), _held(x).to(t))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("m,k,n", [(70, 96, 16), (70, 45, 7), (3000, 64, 256), (700, 320, 64)])
+def test_linear_gradients_at_the_largest_values(monkeypatch, dtype, act, m, k, n):
+    monkeypatch.setattr(_token_ops, "checkpoint", _held)
+    x = _top_rows(m, k, dtype).requires_grad_(True)
+    w = _rand(n, k, seed=1, dtype=dtype, scale=2.0 ** -9).requires_grad_(True)
+    b = _rand(n, seed=2, dtype=dtype).requires_grad_(True)
+    dy = _rand(m, n, seed=3, dtype=dtype, scale=2.0 ** -9)
+    dy[1] = 0  # 0 times a finite value
+    y = ops.linear_ckpt8(x, w, b, act=act)
+    y.backward(dy)
+    ref = LinearRef(x, w, b, act, dy)
+    check(y, ref.y, ref.y_tol, "y")
+    check(x.grad, ref.dx, ref.dx_tol, "dx")
+    check(w.grad, ref.dw, ref.dw_tol, "dw")
+    check(b.grad, ref.db, ref.db_tol, "db")
+
+
+@pytest.mark.parametrize("c", [64, 45, 520, 2056])
+def test_layer_norm_gradients_at_the_largest_values(monkeypatch, c):
+    monkeypatch.setattr(_token_ops, "checkpoint", lambda s: _held(s, F16))  # NormRef has s in fp64
+    x = _top_rows(20, c, F16).requires_grad_(True)  # the variance is a number in fp32
+    w, b = (1 + _rand(c, seed=1, scale=0.2)).requires_grad_(True), _rand(c, seed=2).requires_grad_(True)
+    dy = _rand(20, c, seed=3, dtype=F16)
+    y = ops.layer_norm(x, w, b, ckpt8=True)
+    y.backward(dy)
+    ref = NormRef(x, w, b, 1e-5, None, F16, dy, None, True)
+    check(y, ref.y, ref.y_tol, "y")
+    check(x.grad, ref.dx, ref.dx_tol(F16), "dx")
+    check(w.grad, ref.dw, ref.dw_tol, "dw")
+    check(b.grad, ref.db, ref.db_tol, "db")
+    for t in (F32, BF16):  # it is infinite: rstd = 0, and so is the gradient of that row
+        x = _top_rows(20, c, t).requires_grad_(True)
+        ops.layer_norm(x, w, b, ckpt8=True).backward(dy.to(t))
+        assert torch.isfinite(x.grad).all() and not x.grad[1].any()
