@@ -115,13 +115,18 @@ def ckpt8_saved(x: Optional[torch.Tensor]):
 
     def pack(t):
         if (t.dtype, t.numel(), t.data_ptr(), t.device) != who or isinstance(t, nn.Parameter):
-            return t
+            return t, t._version  # autograd leaves the check for changes in place to the hooks
         last = t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last) and not t.is_contiguous()
         return last, ckpt8_pack(t.permute(0, 2, 3, 1) if last else t)
 
     def unpack(held):
-        if isinstance(held, torch.Tensor):
-            return held
+        if isinstance(held[0], torch.Tensor):
+            t, version = held
+            if t._version != version:
+                raise RuntimeError(
+                    "ckpt8_saved: one of the variables needed for gradient computation has been modified by an inplace "
+                    f"operation: a tensor of shape {tuple(t.shape)} is at version {t._version}, expected version {version}")
+            return t
         last, ckpt = held
         v = ckpt8_unpack(ckpt)
         return v.permute(0, 3, 1, 2) if last else v

@@ -73,3 +73,30 @@ def test_layer_norm_gradients_at_the_largest_values(monkeypatch):
     ref = NormRef(x, w, None, 1e-5, None, torch.float16, dy, None, True)
     check(x.grad, ref.dx, ref.dx_tol(torch.float16), "dx")
     check(w.grad, ref.dw, ref.dw_tol, "dw")
+
+
+# ------------------------------------------------------------------------------- ckpt8_saved
+
+
+def test_ckpt8_saved_notices_a_change_in_place_of_what_it_leaves_alone():
+    x = _rand(2, 8, 5, 6).requires_grad_(True)
+    conv = torch.nn.Conv2d(8, 8, 3, padding=1, groups=8)
+    with ops.ckpt8_saved(x):
+        y = conv(x)
+    with torch.no_grad():
+        conv.weight.add_(1)  # as an optimizer does
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with ops.ckpt8_saved(x):
+        z = torch.sigmoid(conv(x))  # saves its result
+    z.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    a = x * 1
+    with ops.ckpt8_saved(a):
+        y = conv(a)
+    a.zero_()  # the checkpoint is of the values at the time
+    (got,) = torch.autograd.grad(y.square().sum(), conv.weight)
+    with ops.ckpt8_saved(x):
+        y = conv(x)
+    assert torch.equal(got, torch.autograd.grad(y.square().sum(), conv.weight)[0])
