@@ -105,7 +105,7 @@ def ckpt8_saved(x: Optional[torch.Tensor]):
     held as an 8-bit checkpoint and decoded when the backward asks for it; every other saved tensor
     stays as it is.  4-D channels-last tensors are blocked along their channels, others along the last
     axis.  ``None``, a tensor of another type, or one that carries no gradient: nothing changes."""
-    if x is None or x.dtype not in _DTYPES or not (torch.is_grad_enabled() and x.numel()):
+    if x is None or x.dtype not in _DTYPES or not (torch.is_grad_enabled() and x.requires_grad and x.numel()):
         yield
         return
 

@@ -100,3 +100,15 @@ def test_ckpt8_saved_notices_a_change_in_place_of_what_it_leaves_alone():
     with ops.ckpt8_saved(x):
         y = conv(x)
     assert torch.equal(got, torch.autograd.grad(y.square().sum(), conv.weight)[0])
+
+
+def test_ckpt8_saved_leaves_an_input_without_a_gradient_alone():
+    x, w, dy = _rand(4, 32), _rand(5, 32, seed=1).requires_grad_(True), _rand(4, 5, seed=2)
+    want = torch.autograd.grad(torch.nn.functional.linear(x, w), w, dy)[0]
+    with ops.ckpt8_saved(x):
+        y = torch.nn.functional.linear(x, w)
+    assert torch.equal(torch.autograd.grad(y, w, dy)[0], want)
+    x.requires_grad_(True)
+    with ops.ckpt8_saved(x):
+        y = torch.nn.functional.linear(x, w)
+    assert not torch.equal(torch.autograd.grad(y, w, dy)[0], want)
