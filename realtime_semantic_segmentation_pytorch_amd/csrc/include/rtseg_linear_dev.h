@@ -37,16 +37,17 @@ __device__ __forceinline__ float normal_tail(float a) {
   return __builtin_amdgcn_exp2f(__builtin_fmaf(a, q, -0.9999992251396179f));
 }
 // gelu(x) = x Phi(x) = max(x, 0) - |x| Phi(-|x|), gelu'(x) = Phi(x) + x phi(x).  16-bit operands take the tail
-// above (11 full-rate instructions and one quarter-rate; erff costs five times that, and the activation is
+// above (10 full-rate instructions and one quarter-rate; erff costs five times that, and the activation is
 // what bounds the wide layers' forward); fp32 ones erff.  max and min work on the bits: the float forms
 // spend an instruction each to quiet a NaN, which here comes through the tail.
 template <typename T>
 __device__ __forceinline__ float gelu(float x) {
   if constexpr (sizeof(T) == 4) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
   const int bits = __float_as_int(x);
-  // the factor is cut off at 64, where the tail is 0: inf - inf * 0 is inf
-  const float a = __int_as_float(min(bits & 0x7fffffff, 0x42800000));
-  return __builtin_fmaf(-a, normal_tail(fabsf(x)), __int_as_float(max(bits, 0)));
+  // The factor of a positive x is cut off at 64, where the tail is 0: gelu(inf) = inf - 64 * 0.  As integers the
+  // negative ones are below that and pass: gelu(-inf) = -inf * 0, a NaN as in every other form.
+  const float a = __int_as_float(min(bits, 0x42800000));
+  return __builtin_fmaf(-fabsf(a), normal_tail(fabsf(x)), __int_as_float(max(bits, 0)));
 }
 template <typename T>
 __device__ __forceinline__ float gelu_slope(float x) {

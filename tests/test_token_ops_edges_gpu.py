@@ -93,3 +93,22 @@ def test_layer_norm_gradients_at_the_largest_values(monkeypatch, c):
         x = _top_rows(20, c, t).requires_grad_(True)
         ops.layer_norm(x, w, b, ckpt8=True).backward(dy.to(t))
         assert torch.isfinite(x.grad).all() and not x.grad[1].any()
+
+
+# ------------------------------------------------------------------------------- infinities
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [32, 33])
+def test_gelu_of_infinities_and_nan_is_the_stock_one(dtype, n):
+    """One row each: gelu(-inf) = -inf * 0 is NaN in every type."""
+    x = torch.zeros(6, n, device="cuda", dtype=dtype)
+    at = torch.tensor([float("-inf"), float("inf"), float("nan"), float("nan"), torch.finfo(dtype).min, torch.finfo(dtype).max])
+    x[torch.arange(6), 0] = at.to("cuda", dtype)
+    x[3, 0] = -x[3, 0]  # a NaN with its sign set
+    w = torch.zeros(n, n, device="cuda", dtype=dtype)
+    w[0, 0] = 1.0
+    got = ops.linear_ckpt8(x, w, None, act="gelu")[:, 0]
+    want = torch.nn.functional.gelu(x[:, 0].float()).to(dtype)
+    assert torch.isnan(want[[0, 2, 3]]).all()
+    torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
