@@ -205,8 +205,10 @@ def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise ValueError(f"linear_ckpt8: bias must have shape ({weight.shape[0]},), got {tuple(bias.shape)}")
     kind = x.device.type
-    if torch.is_autocast_enabled(kind):
+    if torch.is_autocast_enabled(kind) and x.dtype in _DTYPES:  # autocast leaves fp64 alone
         x = x.to(torch.get_autocast_dtype(kind))
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"linear_ckpt8: fp32, bf16 or fp16 expected, got {x.dtype}")
     if bias is not None and bias.dtype != weight.dtype:
         raise TypeError(f"linear_ckpt8: weight and bias must be of one type, got {weight.dtype} and {bias.dtype}")
     if weight.dtype not in (x.dtype, torch.float32):
@@ -214,8 +216,6 @@ def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     for p in (weight, bias):
         if p is not None and p.device != x.device:
             raise ValueError(f"linear_ckpt8: all tensors must be on one device, got {x.device} and {p.device}")
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"linear_ckpt8: fp32, bf16 or fp16 expected, got {x.dtype}")
     if use_hip(x, "ckpt8"):
         return ops().linear_ckpt8(x, weight, bias, ACTS[act])
     y = _LinearCkpt8Fn.apply(_rows(x, "linear_ckpt8"), weight, bias, act)

@@ -112,3 +112,16 @@ def test_ckpt8_saved_leaves_an_input_without_a_gradient_alone():
     with ops.ckpt8_saved(x):
         y = torch.nn.functional.linear(x, w)
     assert not torch.equal(torch.autograd.grad(y, w, dy)[0], want)
+
+
+# ------------------------------------------------------------------------------- types
+
+
+def test_linear_refuses_fp64_and_integers_under_autocast_too():
+    w = _rand(3, 8)
+    for x in (_rand(4, 8).double(), torch.ones(4, 8, dtype=torch.int32)):
+        for on in (False, True):
+            with torch.autocast("cpu", dtype=torch.bfloat16, enabled=on):
+                for weight in (w, w.to(x.dtype)):
+                    with pytest.raises(TypeError, match="fp32, bf16 or fp16 expected"):
+                        ops.linear_ckpt8(x, weight)
