@@ -55,7 +55,8 @@ def _add_norm(norm, x, branch=None, cast=True, want_sum=True):
     the linear layers behind it run in (``cast``; autocast would convert it there)."""
     if isinstance(norm, ops.LayerNorm) and (x.is_cuda or norm.ckpt8):
         kind = x.device.type
-        out = torch.get_autocast_dtype(kind) if cast and torch.is_autocast_enabled(kind) else None
+        cast = cast and x.dtype != torch.float64 and torch.is_autocast_enabled(kind)
+        out = torch.get_autocast_dtype(kind) if cast else None
         if branch is None:
             return x, norm(x, out_dtype=out)
         return norm(x, residual=branch, out_dtype=out, want_sum=want_sum)

@@ -31,8 +31,8 @@ def _autocast_dtype(t: torch.Tensor) -> Optional[torch.dtype]:
 
 
 def _default_out(x: torch.Tensor) -> torch.dtype:
-    """What ``F.layer_norm`` returns: fp32 under autocast, else the input's type."""
-    return torch.float32 if _autocast_dtype(x) is not None else x.dtype
+    """What ``F.layer_norm`` returns: fp32 under autocast, which leaves fp64 alone, else the input's type."""
+    return torch.float32 if x.dtype != torch.float64 and _autocast_dtype(x) is not None else x.dtype
 
 
 def layer_norm_reference(x, weight=None, bias=None, eps=1e-5, residual=None, out_dtype=None):
@@ -92,7 +92,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     ``x``: ``[..., C]`` fp32 / bf16 / fp16, any strides (a non-contiguous one is copied once).  ``s``
     has the promoted type of ``x`` and ``residual``; ``y`` has ``out_dtype``, by default fp32 under
-    autocast and the type of ``s`` otherwise (as ``F.layer_norm``).  ``weight`` / ``bias``: ``[C]`` or
+    autocast (fp64 stays fp64) and the type of ``s`` otherwise (as ``F.layer_norm`` on the GPU).  ``weight`` / ``bias``: ``[C]`` or
     None, applied in fp32.  ``ckpt8``: hold ``s`` for the backward in 8 bits; the backward then uses
     the checkpoint's values in place of ``s`` (with the exact mean and variance).
     """

@@ -125,3 +125,13 @@ def test_linear_refuses_fp64_and_integers_under_autocast_too():
                 for weight in (w, w.to(x.dtype)):
                     with pytest.raises(TypeError, match="fp32, bf16 or fp16 expected"):
                         ops.linear_ckpt8(x, weight)
+
+
+def test_layer_norm_of_fp64_stays_fp64_under_autocast():
+    x, m = _rand(4, 8).double(), torch.nn.LayerNorm(8).double()
+    ops.convert_layernorm(torch.nn.Sequential(m))
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        ref = torch.nn.functional.layer_norm(x, (8,), m.weight, m.bias)
+        s, y = m(x, residual=torch.zeros_like(x))
+        assert ref.dtype == ops.layer_norm(x).dtype == y.dtype == s.dtype == torch.float64
+    torch.testing.assert_close(y, ref, rtol=1e-14, atol=1e-14)  # a few of fp64's roundings
