@@ -135,3 +135,12 @@ def test_layer_norm_of_fp64_stays_fp64_under_autocast():
         s, y = m(x, residual=torch.zeros_like(x))
         assert ref.dtype == ops.layer_norm(x).dtype == y.dtype == s.dtype == torch.float64
     torch.testing.assert_close(y, ref, rtol=1e-14, atol=1e-14)  # a few of fp64's roundings
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.bool, torch.complex64])
+def test_layer_norm_refuses_what_is_no_float(dtype):
+    x = torch.ones(4, 8, dtype=dtype)
+    with pytest.raises(TypeError, match="x must be of a floating type"):
+        ops.layer_norm(x)
+    with pytest.raises(TypeError, match="residual must be of a floating type"):
+        ops.layer_norm(torch.ones(4, 8), residual=x)
