@@ -175,14 +175,15 @@ class _LinearCkpt8Fn(torch.autograd.Function):
         dx = dw = db = None
         z = None if codes is None else _unpack_reference(codes, scales, ctx.k, torch.float32, dy.dtype)
         g = dy.float()
-        if need_x:
-            dx = g @ weight.to(dy.dtype).float()
-            dx = (dx * _gelu_slope(z) if ctx.act == "gelu" else dx).to(dy.dtype)
-        if need_w:
-            a = _gelu(z).to(dy.dtype).float() if ctx.act == "gelu" else z
-            dw = (g.t() @ a).to(ctx.wtype)
-        if need_b:
-            db = g.sum(0).to(ctx.wtype)
+        with torch.autocast(dy.device.type, enabled=False):  # the backward may be called inside of one
+            if need_x:
+                dx = g @ weight.to(dy.dtype).float()
+                dx = (dx * _gelu_slope(z) if ctx.act == "gelu" else dx).to(dy.dtype)
+            if need_w:
+                a = _gelu(z).to(dy.dtype).float() if ctx.act == "gelu" else z
+                dw = (g.t() @ a).to(ctx.wtype)
+            if need_b:
+                db = g.sum(0).to(ctx.wtype)
         return dx, dw, db, None
 
 

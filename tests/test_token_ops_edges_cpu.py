@@ -144,3 +144,14 @@ def test_layer_norm_refuses_what_is_no_float(dtype):
         ops.layer_norm(x)
     with pytest.raises(TypeError, match="residual must be of a floating type"):
         ops.layer_norm(torch.ones(4, 8), residual=x)
+
+
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_linear_gradients_inside_autocast_are_those_outside(act):
+    x, w, b = (t.requires_grad_(True) for t in (_rand(8, 64), _rand(16, 64, seed=1), _rand(16, seed=2)))
+    dy = _rand(8, 16, seed=3)
+    want = torch.autograd.grad(ops.linear_ckpt8(x, w, b, act=act), (x, w, b), dy)
+    y = ops.linear_ckpt8(x, w, b, act=act)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = torch.autograd.grad(y, (x, w, b), dy)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
