@@ -26,6 +26,7 @@ import math
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 
 from ... import ops
 
@@ -50,10 +51,17 @@ def _drop_path(x, p, training):
     return x * mask / keep
 
 
+def _watched(m):
+    """Whether somebody reads or replaces what ``m`` is called with and returns: hooks, a ``forward`` of the
+    instance's own.  Such a module is called as the stock model calls it, outside of any fusion."""
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                or "forward" in m.__dict__ or _has_any_global_hook())
+
+
 def _add_norm(norm, x, branch=None, cast=True, want_sum=True):
     """``(s, norm(s))`` for ``s = x + branch``; on the HIP kernel one pass, whose result has the type that
     the linear layers behind it run in (``cast``; autocast would convert it there)."""
-    if isinstance(norm, ops.LayerNorm) and (x.is_cuda or norm.ckpt8):
+    if type(norm) is ops.LayerNorm and (x.is_cuda or norm.ckpt8) and not _watched(norm):
         kind = x.device.type
         cast = cast and x.dtype != torch.float64 and torch.is_autocast_enabled(kind)
         out = torch.get_autocast_dtype(kind) if cast else None
@@ -98,7 +106,8 @@ class Mlp(nn.Module):
 
     def forward(self, x, h, w):
         x = self.dwconv(self.fc1(x), h, w)
-        if isinstance(self.fc2, ops.Ckpt8Linear) and isinstance(self.act, nn.GELU) and self.act.approximate == "none":
+        if (type(self.fc2) is ops.Ckpt8Linear and isinstance(self.act, nn.GELU) and self.act.approximate == "none"
+                and not (_watched(self.fc2) or _watched(self.act))):
             return self.fc2(x, act="gelu")
         return self.fc2(self.act(x))
 
@@ -146,13 +155,16 @@ class Block(nn.Module):
         self.norm2 = nn.LayerNorm(dim, eps=1e-6)
         self.mlp = Mlp(dim, dim * 4)
 
-    def forward(self, x, h, w, branch=None, split=False):
-        """``branch`` is added to ``x`` first; ``split`` returns (stream, its last branch) unadded, so
-        that the next norm adds them."""
+    def parts(self, x, h, w, branch=None):
+        """The stream and its last branch, unadded, so that the next norm adds them; ``branch`` (the last
+        block's) is added to ``x`` first."""
         x, y = _add_norm(self.norm1, x, branch)
         x, y = _add_norm(self.norm2, x, self.drop_path(self.attn(y, h, w)))
-        branch = self.drop_path(self.mlp(y, h, w))
-        return (x, branch) if split else x + branch
+        return x, self.drop_path(self.mlp(y, h, w))
+
+    def forward(self, x, h, w):
+        x, branch = self.parts(x, h, w)
+        return x + branch
 
 
 class OverlapPatchEmbed(nn.Module):
@@ -202,7 +214,10 @@ class MixVisionTransformerEncoder(nn.Module):
             x, h, w = getattr(self, f"patch_embed{i}")(x)
             branch = None
             for blk in getattr(self, f"block{i}"):
-                x, branch = blk(x, h, w, branch, True)
+                if type(blk) is Block and not _watched(blk):
+                    x, branch = blk.parts(x, h, w, branch)
+                else:
+                    x, branch = blk(x if branch is None else x + branch, h, w), None
             _, x = _add_norm(getattr(self, f"norm{i}"), x, branch, cast=False, want_sum=False)
             x = x.reshape(b, h, w, -1).permute(0, 3, 1, 2).contiguous()
             outs.append(x)

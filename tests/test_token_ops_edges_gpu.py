@@ -6,6 +6,7 @@ import torch
 import _token_ops
 from _token_ops import LinearRef, NormRef, check
 from realtime_semantic_segmentation_pytorch_amd import ops
+from realtime_semantic_segmentation_pytorch_amd.models.smp import get_encoder
 from realtime_semantic_segmentation_pytorch_amd.ops.ckpt8 import _pack_reference
 
 pytestmark = pytest.mark.gpu
@@ -112,3 +113,34 @@ def test_gelu_of_infinities_and_nan_is_the_stock_one(dtype, n):
     want = torch.nn.functional.gelu(x[:, 0].float()).to(dtype)
     assert torch.isnan(want[[0, 2, 3]]).all()
     torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
+
+
+# ------------------------------------------------------------------------------- hooks of a Mix Transformer
+
+
+@pytest.mark.parametrize("convert", [ops.convert_layernorm, ops.convert_ckpt8])
+@pytest.mark.parametrize("amp", [False, True])
+def test_hooks_of_a_mit_see_the_stock_tensors(convert, amp):
+    torch.manual_seed(0)
+    e, x = get_encoder("mit_b0").cuda().eval(), _rand(1, 3, 64, 64)
+    ref, seen = [], []
+
+    def run(into):
+        with torch.autocast("cuda", dtype=BF16, enabled=amp):
+            hooks = [m.register_forward_hook(lambda m, args, out, n=n: into.append((n, args[0].detach(), out.detach())))
+                     for n, m in e.named_modules()
+                     if n.count(".") == 1 and n.startswith("block") or n.endswith(("norm1", "norm2", "norm3", "mlp.act", "mlp.fc2"))]
+            out = e(x)
+            for h in hooks:
+                h.remove()
+            return out, e(x)
+
+    want = run(ref)
+    convert(e)
+    got = run(seen)
+    assert [n for n, _, _ in seen] == [n for n, _, _ in ref] and "block1.0.mlp.act" in {n for n, _, _ in seen}
+    tol = 3e-2 if amp else 1e-4  # bf16 products in another order, 2^-8 a rounding over 8 blocks; fp32 sums in another order
+    for a, b in [(p[i], q[i]) for p, q in zip(seen, ref) for i in (1, 2)] + [pq for g, w in zip(got, want) for pq in zip(g, w)]:
+        assert a.shape == b.shape and a.dtype == b.dtype
+        if a.numel():
+            assert float((a.float() - b.float()).norm() / b.float().norm()) < tol
