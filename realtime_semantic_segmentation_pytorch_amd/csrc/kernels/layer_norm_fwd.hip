@@ -68,17 +68,25 @@ __global__ void __launch_bounds__(kThreads) ln_fwd_kernel(const LnFwdArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += v[j][i];  // channels past C were loaded as 0
   const float inv_c = 1.f / static_cast<float>(a.C);
-  const float mean = row_sum<BLOCK>(sum, G, red, turn) / static_cast<float>(a.C);  // exact for a constant row
-  float sq = 0.f;
+  // The sum's roundings leave the mean off by up to 41 of its own; the differences from it, small and nearly exact where
+  // that matters, give back what is missing: the mean of equal values is that value, and a row of a large mean keeps
+  // its digits.  The variance is taken around the first mean and moved by the square of the second.
+  const float first_mean = row_sum<BLOCK>(sum, G, red, turn) * inv_c;
+  float sd = 0.f, sq = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float d = v[j][i] - mean;
-      sq += (VEC ? n[j] > 0 : i < n[j]) ? d * d : 0.f;
+      const float d = (VEC ? n[j] > 0 : i < n[j]) ? v[j][i] - first_mean : 0.f;
+      sd += d;
+      sq += d * d;
     }
   }
-  const float rstd = 1.f / sqrtf(row_sum<BLOCK>(sq, G, red, turn) * inv_c + a.eps);
+  const float rest = row_sum<BLOCK>(sd, G, red, turn) * inv_c;
+  const float mean = first_mean + rest;
+  // fused: the square, of no more than the other term, is not rounded to an infinity by itself
+  const float var = fmaxf(__builtin_fmaf(-rest, rest, row_sum<BLOCK>(sq, G, red, turn) * inv_c), 0.f);
+  const float rstd = 1.f / sqrtf(var + a.eps);
 
   if (live && lane == 0 && a.mean != nullptr) {
     a.mean[r0 + rl] = mean;

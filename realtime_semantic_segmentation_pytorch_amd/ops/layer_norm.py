@@ -55,6 +55,7 @@ class _LayerNormCkptFn(torch.autograd.Function):
 
         wide = s.detach().float()
         mean = wide.mean(-1, keepdim=True)
+        mean = mean + (wide - mean).mean(-1, keepdim=True)  # what the sum's roundings left out, as in the kernel
         rstd = torch.rsqrt((wide - mean).square().mean(-1, keepdim=True) + eps)
         h = (wide - mean) * rstd
         if weight is not None:

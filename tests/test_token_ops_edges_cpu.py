@@ -221,3 +221,15 @@ def test_a_replaced_block_of_a_mit_is_called_as_the_stock_one():
     calls = []
     e.block2[1].forward = lambda x, h, w: calls.append(1) or stock(x, h, w)
     assert all(torch.equal(a, b) for a, b in zip(e(x), want)) and calls
+
+
+# ------------------------------------------------------------------------------- rows without a variance
+
+
+@pytest.mark.parametrize("c", [7, 48, 161, 320, 4101])
+@pytest.mark.parametrize("value", [1000.1, 0.1, 3333.3333])
+def test_a_constant_row_has_no_variance(c, value):
+    b = _rand(c, seed=1)
+    for ckpt in (False, True):
+        y = ops.layer_norm(torch.full((5, c), value).requires_grad_(True), None, b, 1e-6, ckpt8=ckpt)
+        assert torch.equal(y, b.expand(5, c))

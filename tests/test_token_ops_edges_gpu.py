@@ -144,3 +144,36 @@ def test_hooks_of_a_mit_see_the_stock_tensors(convert, amp):
         assert a.shape == b.shape and a.dtype == b.dtype
         if a.numel():
             assert float((a.float() - b.float()).norm() / b.float().norm()) < tol
+
+
+# ------------------------------------------------------------------------------- rows without a variance
+
+
+@pytest.mark.parametrize("c", [1, 7, 48, 64, 161, 320, 512, 520, 2056, 4101, 8192])
+@pytest.mark.parametrize("value", [1000.1, -1000.1, 0.1, 3333.3333, 1e-3])
+def test_a_constant_row_has_no_variance(c, value):
+    """The mean of equal values is that value: with a mean that is 41 roundings off, 1000.1 would come out as 0.18
+    behind eps = 1e-6."""
+    b = _rand(c, seed=1)
+    for t in (F32, BF16):
+        x = torch.full((5, c), value, device="cuda", dtype=t)
+        for ckpt in (False, True):
+            leaf = x.clone().requires_grad_(True)
+            y = ops.layer_norm(leaf, None, b, 1e-6, out_dtype=F32, ckpt8=ckpt)
+            assert torch.equal(y, b.expand(5, c))
+        assert not ops.layer_norm(x, None, None, 1e-6).any()
+        s, y = ops.layer_norm(x, None, None, 1e-6, residual=torch.full_like(x, 3 * value))
+        assert not y.any()
+
+
+@pytest.mark.parametrize("c", [48, 161, 320, 2056])
+def test_rows_of_a_large_mean(c):
+    """A mean within two roundings of itself, u |mean| each, instead of 41: h is off by 2 u A rstd and rstd's 30 u |h|
+    (_token_ops.NormRef), the products and the bias by 3 u |y|."""
+    x = _rand(64, c, scale=0.05) + 1000.1
+    ref = NormRef(x, None, None, 1e-6)
+    s = x.double()
+    rstd = 1 / torch.sqrt(s.var(1, correction=0, keepdim=True) + 1e-6)
+    u = 2.0 ** -24
+    tol = 2 * u * s.abs().amax(1, keepdim=True) * rstd + 33 * u * ref.y.abs()
+    check(ops.layer_norm(x, None, None, 1e-6), ref.y, tol, "y")
