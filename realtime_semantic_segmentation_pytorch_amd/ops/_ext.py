@@ -14,6 +14,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import build as _build
 
@@ -91,6 +92,15 @@ def use_hip(t: torch.Tensor, family: str | None = None) -> bool:
             "rtseg HIP extension is required for GPU tensors but failed to load: "
             f"{_load_error!r}. Build it with `python -m realtime_semantic_segmentation_pytorch_amd.ops.build`.")
     return True
+
+
+def transformed(t: torch.Tensor) -> bool:
+    """Whether an op on ``t`` is recorded or transformed rather than run: ``torch.jit.trace`` and ONNX export,
+    ``torch.compile`` / ``torch.export``, ``torch.func`` transforms, forward-mode differentiation, tensor
+    subclasses (fake tensors).  A HIP kernel is opaque to all of them; the ops that take the stock operators'
+    place by default run their PyTorch formulation there."""
+    return (type(t) not in (torch.Tensor, torch.nn.Parameter) or torch.compiler.is_compiling() or torch.jit.is_tracing()
+            or torch._C._functorch.peek_interpreter_stack() is not None or forward_ad._current_level >= 0)
 
 
 def differentiable_once(backward):

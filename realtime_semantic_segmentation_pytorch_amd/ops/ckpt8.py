@@ -32,7 +32,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._ext import differentiable_once, ops, use_hip
+from ._ext import differentiable_once, ops, transformed, use_hip
 
 BLOCK = 32
 ACTS = {"none": 0, "gelu": 1}
@@ -104,8 +104,10 @@ def ckpt8_saved(x: Optional[torch.Tensor]):
     """Inside, whatever an operator saves of ``x`` for its backward -- ``x`` or a view of all of it -- is
     held as an 8-bit checkpoint and decoded when the backward asks for it; every other saved tensor
     stays as it is.  4-D channels-last tensors are blocked along their channels, others along the last
-    axis.  ``None``, a tensor of another type, or one that carries no gradient: nothing changes."""
-    if x is None or x.dtype not in _DTYPES or not (torch.is_grad_enabled() and x.requires_grad and x.numel()):
+    axis.  ``None``, a tensor of another type, one that carries no gradient, or a call that is traced or
+    transformed: nothing changes."""
+    if (x is None or x.dtype not in _DTYPES or not (torch.is_grad_enabled() and x.requires_grad and x.numel())
+            or transformed(x)):
         yield
         return
 
@@ -197,7 +199,8 @@ def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     ``"gelu"`` (the erf form, applied in fp32 and rounded to ``x``'s type, as a layer of its own would).
     The value is that of the exact ``x``; the gradients are the formula's at the checkpoint's values:
     ``dx = (dy @ weight) * act'(z)``, ``dweight = dy.T @ act(z)``, ``dbias = dy.sum(rows)``.
-    Without gradients nothing is kept."""
+    Without gradients nothing is kept.  A call that is traced, compiled or transformed (``torch.func``, forward
+    mode) takes the formula itself, without a checkpoint."""
     if act not in ACTS:
         raise ValueError(f"linear_ckpt8: act must be one of {sorted(ACTS)}, got {act!r}")
     if weight.dim() != 2 or min(weight.shape) < 1 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
@@ -217,6 +220,9 @@ def linear_ckpt8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
     for p in (weight, bias):
         if p is not None and p.device != x.device:
             raise ValueError(f"linear_ckpt8: all tensors must be on one device, got {x.device} and {p.device}")
+    if transformed(x):  # traced, compiled, torch.func, forward mode: the formulation itself, without a checkpoint
+        y = linear_ckpt8_reference(_rows(x, "linear_ckpt8"), weight, bias, act)
+        return y.view(*x.shape[:-1], weight.shape[0])
     if use_hip(x, "ckpt8"):
         return ops().linear_ckpt8(x, weight, bias, ACTS[act])
     y = _LinearCkpt8Fn.apply(_rows(x, "linear_ckpt8"), weight, bias, act)

@@ -9,7 +9,8 @@ atomics: the same bits on every run).
 
 ``ckpt8=True`` holds the normalised tensor for the backward as an 8-bit checkpoint (``ops.ckpt8``)
 instead of the tensor itself.  CPU tensors, ``RTSEG_DISABLE_HIP=1`` / ``RTSEG_HIP_OFF=layer_norm``
-and more than 8192 channels run the same formulas in PyTorch.
+and more than 8192 channels run the same formulas in PyTorch; so does a call that is traced, compiled or
+transformed (``torch.func``, forward mode), without a checkpoint.
 """
 from __future__ import annotations
 
@@ -19,7 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from ._ext import differentiable_once, ops, use_hip
+from ._ext import differentiable_once, ops, transformed, use_hip
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _MAX_CHANNELS = 8192  # a row is held in one block's registers
@@ -118,13 +119,14 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
         if residual.dtype != wide and not (wide == torch.float32 and residual.dtype in _DTYPES):
             residual = residual.to(wide)
     out_dtype = out_dtype or _default_out(x)
-    if x.dtype in _DTYPES and out_dtype in _DTYPES and c <= _MAX_CHANNELS and use_hip(x, "layer_norm"):
+    stock = transformed(x)
+    if not stock and x.dtype in _DTYPES and out_dtype in _DTYPES and c <= _MAX_CHANNELS and use_hip(x, "layer_norm"):
         # 16 bits in and another 16-bit type out: through fp32
         got = out_dtype if out_dtype == x.dtype or torch.float32 in (out_dtype, x.dtype) else torch.float32
         *s, y = ops().layer_norm(x, residual, weight, bias, eps, got, ckpt8, residual is not None and want_sum)
         y = y if got == out_dtype else y.to(out_dtype)
         return y if residual is None else (s[0] if s else None, y)
-    if ckpt8 and x.dtype in _DTYPES and torch.is_grad_enabled():
+    if ckpt8 and not stock and x.dtype in _DTYPES and torch.is_grad_enabled():
         s = x if residual is None else x + residual
         y = _LayerNormCkptFn.apply(s, weight, bias, float(eps), out_dtype)
         return y if residual is None else (s if want_sum else None, y)
