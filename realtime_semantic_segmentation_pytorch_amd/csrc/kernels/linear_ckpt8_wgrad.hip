@@ -358,8 +358,11 @@ void launch_tn(TnArgs p, const TnPlan& w, bool vec, hipStream_t st) {
     case 64: vec ? go(lin_tn_kernel<T, ACT, 1, 4, 2, 4, true, 4 - F>, 256) : go(lin_tn_kernel<T, ACT, 1, 4, 2, 4, false, 2>, 256); break;
     case 128: vec ? go(lin_tn_kernel<T, ACT, 2, 2, 4, 4, true, 3>, 256) : go(lin_tn_kernel<T, ACT, 2, 2, 4, 4, false, 2>, 256); break;
     case 256: vec ? go(lin_tn_kernel<T, ACT, 4, 1, 4, 4, true, ACT == kCkptGelu ? 2 : 3 - F>, 256) : go(lin_tn_kernel<T, ACT, 4, 1, 4, 4, false, 2>, 256); break;
-    case 320: vec ? go(lin_tn_kernel<T, ACT, 4, 1, 4, 5, true, 2>, 256) : go(lin_tn_kernel<T, ACT, 4, 1, 4, 5, false, 2>, 256); break;
-    default: vec ? go(lin_tn_kernel<T, ACT, 8, 1, 4, 4, true, 2>, 512) : go(lin_tn_kernel<T, ACT, 8, 1, 4, 4, false, 2>, 512); break;
+    default:  // behind gelu alone
+      if constexpr (ACT == kCkptGelu) {
+        if (w.cols == 320) vec ? go(lin_tn_kernel<T, ACT, 4, 1, 4, 5, true, 2>, 256) : go(lin_tn_kernel<T, ACT, 4, 1, 4, 5, false, 2>, 256);
+        else vec ? go(lin_tn_kernel<T, ACT, 8, 1, 4, 4, true, 2>, 512) : go(lin_tn_kernel<T, ACT, 8, 1, 4, 4, false, 2>, 512);
+      }
   }
 }
 
