@@ -1,9 +1,10 @@
-"""The checkpointing linear layer on the GPU against 64 bits at sizes that reach every tile of its three kernels
-(csrc/kernels/linear_ckpt8_*.hip), in every type: a full tile, a ragged one and an unaligned one of each."""
+"""The token operators on the GPU against 64 bits at sizes that reach every tile of the checkpointing linear layer's
+three kernels (csrc/kernels/linear_ckpt8_*.hip) and every layout of a row in the layer norm's, in every type."""
 import pytest
 import torch
 
 from _token_ops import LinearRef, check
+from test_layer_norm_gpu import _run as run_norm
 from realtime_semantic_segmentation_pytorch_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -46,6 +47,9 @@ SIZES = [
     (8300, 129, 300),    # ... its 320 columns
     (16411, 31, 97),     # ... its 128 columns
     (16411, 45, 63),     # ... its 64 columns
+    (16411, 64, 24),     # fp32, one step: data gradient 64 columns
+    (16411, 128, 24),    # ... 128 columns
+    (16411, 32, 104),    # ... forward 128 columns
     (16411, 64, 257),    # aligned k, unaligned n: aligned forward, the others not
     (16411, 257, 64),    # unaligned k, aligned n
 ]
@@ -94,3 +98,12 @@ def test_bias_gradient_alone(dtype, m, n):
     ops.linear_ckpt8(x, w, b).backward(dy)
     ref = LinearRef(x, w, b, "none", dy)
     check(b.grad, ref.db, ref.db_tol, "db")
+
+
+@pytest.mark.parametrize("x_t,r_t,out_t", [(F32, None, F32), (F32, BF16, BF16), (F32, F16, F16), (BF16, None, F32), (BF16, BF16, BF16),
+                                           (F16, None, F32), (F16, F16, F16)])
+@pytest.mark.parametrize("c", [40, 45, 64, 320, 161, 1024, 1001, 2016, 1999, 2056, 2053, 4104, 4101])
+def test_norm_layouts(x_t, r_t, out_t, c):
+    """1 .. 4 vectors of 8 channels a lane, a wave's lanes or a block's, aligned and not."""
+    for ckpt in (False, True):
+        run_norm(21, c, x_t, r_t, out_t, ckpt)
