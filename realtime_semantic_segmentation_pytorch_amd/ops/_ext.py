@@ -94,13 +94,18 @@ def use_hip(t: torch.Tensor, family: str | None = None) -> bool:
     return True
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+_is_compiling, _is_tracing = torch.compiler.is_compiling, torch._C._is_tracing
+_func_transform = torch._C._functorch.peek_interpreter_stack
+
+
 def transformed(t: torch.Tensor) -> bool:
     """Whether an op on ``t`` is recorded or transformed rather than run: ``torch.jit.trace`` and ONNX export,
     ``torch.compile`` / ``torch.export``, ``torch.func`` transforms, forward-mode differentiation, tensor
     subclasses (fake tensors).  A HIP kernel is opaque to all of them; the ops that take the stock operators'
     place by default run their PyTorch formulation there."""
-    return (type(t) not in (torch.Tensor, torch.nn.Parameter) or torch.compiler.is_compiling() or torch.jit.is_tracing()
-            or torch._C._functorch.peek_interpreter_stack() is not None or forward_ad._current_level >= 0)
+    return (type(t) not in _PLAIN or _is_compiling() or _is_tracing() or _func_transform() is not None
+            or forward_ad._current_level >= 0)
 
 
 def differentiable_once(backward):

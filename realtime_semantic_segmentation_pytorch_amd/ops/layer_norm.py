@@ -101,9 +101,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     c = x.shape[-1] if x.dim() else 0
     if c < 1:
         raise ValueError(f"layer_norm: the last axis must have at least one channel, got shape {tuple(x.shape)}")
-    for name, t in (("x", x), ("residual", residual)):
-        if t is not None and not t.is_floating_point():
-            raise TypeError(f"layer_norm: {name} must be of a floating type, got {t.dtype}")
+    if not x.is_floating_point():
+        raise TypeError(f"layer_norm: x must be of a floating type, got {x.dtype}")
+    if residual is not None and not residual.is_floating_point():
+        raise TypeError(f"layer_norm: residual must be of a floating type, got {residual.dtype}")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None and tuple(p.shape) != (c,):
             raise ValueError(f"layer_norm: {name} must have shape ({c},), got {tuple(p.shape)}")
