@@ -351,7 +351,8 @@ std::optional<at::Tensor> maybe(const at::Tensor& t) { return t.defined() ? std:
 struct LinearCkpt8Fn : torch::autograd::Function<LinearCkpt8Fn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
                             const std::optional<at::Tensor>& b, int64_t act, bool need_x, bool need_w, bool need_b) {
-    // fp32 weights beside 16-bit operands are cast once, for the forward and the data gradient
+    // fp32 weights beside 16-bit operands are cast once, for the forward and the data gradient, as autocast casts
+    // them (what that costs in digits: rtseg_linear_dev.h)
     const at::Tensor x2 = rows_of(x), wc = w.to(x.scalar_type()).contiguous();
     auto shape = x.sizes().vec();
     if (need_x) ctx->saved_data["shape"] = shape;

@@ -6,8 +6,12 @@
 //   wgrad     dw = dy^T act(z), db = sum_rows dy
 //
 // bf16 / fp16 operands feed v_mfma_f32_16x16x32, fp32 ones v_mfma_f32_16x16x4_f32; sums are fp32.
-// act = gelu is computed in fp32 and rounded to the operands' type in front of the product, which is
-// what a separate activation layer hands to a linear layer.
+// Operands are of x's type, and two are rounded to it: act = gelu, computed in fp32 and rounded in front of the
+// product, and fp32 weights beside a 16-bit x (cast by the caller, binding_ckpt8.cpp).  Both are what a separate
+// activation layer and autocast hand to a linear layer; a second product for the rest of each would double the
+// MFMA work.  Relative to the formula with exact operands, bf16 (fp16: an eighth), 256 to 64: y is off by 2.4e-3
+// with fp32 weights and 2.9e-3 behind gelu as well, of which 1.7e-3 are the rounding of y itself; dw of fp32
+// weights is off by 1.7e-3 behind gelu and by fp32 sums (7e-8) without it, since a checkpoint's values are exact.
 #pragma once
 
 #include "rtseg_ckpt8.h"

@@ -10,8 +10,8 @@
 // What bounds it: HBM (dy is read, the codes, dx written once) and, with gelu, the 20 VALU instructions of
 // act' for every element.  Where n fits one step, w stays in LDS and the block walks down the rows; few
 // tiles split n over 4 groups of waves, joined in LDS in order.  Measured: 131072 x 256 to 64 channels 19 us
-// (84 MB, 4.4 TB/s), 131072 x 64 to 256 with gelu's slope 34 us (118 MB, 3.5 TB/s), 32768 x 320 to 1280 with the
-// slope 75 us (360 TF, 147 MB).
+// (84 MB, 4.4 TB/s), 131072 x 64 to 256 with gelu's slope 33 us (118 MB, 3.6 TB/s), 32768 x 320 to 1280 with the
+// slope 69 us (390 TF, 147 MB).
 #include "rtseg_linear_dev.h"
 
 namespace rtseg {

@@ -14,8 +14,9 @@
 // element is evaluated once -- and latency for small ones: few tiles split k over 4 groups of waves, whose
 // sums are joined in LDS in order.  Weights whose k fits one step stay in registers while the block walks
 // down the rows.  Measured: 131072 x 64 to 256 columns 27 us (93 MB, 3.4 TB/s), 131072 x 256 to
-// 64 with gelu 37 us (3.2 TB/s), 32768 x 1280 to 320 with gelu 91 us (295 TF; waits, not arithmetic: without gelu
-// 88, without the products 92, without the loads of w 65), 2048 x 512 to 2048 15 us (290 TF), 32 x 256 to 256 4 us.
+// 64 with gelu 35 us (118 MB, 3.4 TB/s), 32768 x 1280 to 320 with gelu 86 us (310 TF; waits for w, not arithmetic:
+// in a run of 91 us, 88 without gelu, 92 without the products, 65 without the loads of w), 2048 x 512 to 2048
+// 14.4 us (300 TF; 256 tiles, one block a CU and one wave a SIMD: nothing covers a step's wait), 32 x 256 to 256 4 us.
 #include "rtseg_linear_dev.h"
 
 namespace rtseg {

@@ -6,11 +6,12 @@
 // each MFMA tile).  The row range is split over blocks and the fp32 partial tiles are summed in order by a
 // second kernel: no atomics, the same bits on every run.
 //
-// What bounds it: HBM and, with gelu, the VALU work of decoding.  So a tile is as wide in n as the layer
-// (up to 512), which decodes every code once, and 64 or 128 channels of k; the number of blocks is held near
-// one or two a CU, because each of them writes (and the join reads) one fp32 tile.  Measured with the join:
-// 131072 rows of 256 x 64 21.8 us (76 MB, 3.5 TB/s), of 64 x 256 with gelu 29.8 us, 32768 of 320 x 1280 with gelu
-// 74 us (363 TF).
+// What bounds it: HBM and, with gelu, the VALU work of decoding and of the tail: some 30 instructions an element,
+// 33.5 M elements of 131072 x 256 make 1.0 G lane instructions, 25 us at 256 CUs x 64 lanes x 2.4 GHz.  So with gelu a
+// tile is as wide in n as the layer (up to 512), which decodes every code once, and 64 or 128 channels of k; the
+// number of blocks is held near one or two a CU, because each of them writes (and the join reads) one fp32 tile.
+// Measured, and the join: 131072 rows of 256 x 64 17.3 + 4.3 us (76 MB, 3.5 TB/s), of 64 x 256 with gelu 23.5 + 4.6
+// us, 32768 of 320 x 1280 with gelu 59 + 8 us (400 TF).  The bias gradient alone: 131072 x 64 8.9 + 5.0 us (16.8 MB).
 #include "rtseg_linear_dev.h"
 
 namespace rtseg {
